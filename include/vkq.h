@@ -411,6 +411,183 @@ VKQ_API int vkq_gguf_load_tensor(vkq_gguf *gguf, int64_t index, int device, void
 VKQ_API int vkq_gguf_load_shard(vkq_gguf *gguf, int64_t index, int64_t col_lo, int64_t col_hi, int device,
                                 void *dst, int64_t dst_bytes, void *stream);
 
+/* ---- Serving several sequences: rotary positions, an 8-bit paged KV cache ----
+ * The reference serves one sequence with a float32 cache that it regrows and
+ * copies every token (concatenateSeqDim, internal/transformer/attention.go:
+ * 529-569) and RoPE over interleaved pairs of the whole head (rope.go:49-124).
+ * The entry points below have no counterpart there: they serve many sequences
+ * from one pool of pages, in 8 bits.  None of them allocates device memory. */
+
+/* Element types of activations (the GGML type codes). */
+enum vkq_dtype { VKQ_F32 = 0, VKQ_F16 = 1, VKQ_BF16 = 30 };
+/* Which two values of a head form a pair: (2i, 2i + 1), or (i, i + rot_dim / 2). */
+#define VKQ_ROPE_INTERLEAVED 0
+#define VKQ_ROPE_HALF 1
+
+/* Rotary positions: x [tokens][heads][head_dim], the token and the head at
+ * strides of their own (in elements; a head's values are contiguous), e.g. the
+ * q part of a fused projection's rows.  The first rot_dim values of a head
+ * (even, <= head_dim) are rotated, the others copied:
+ *   out_a = x_a * c - x_b * s,  out_b = x_a * s + x_b * c
+ * with (a, b) the pair of `layout` and c, s = entry [positions[t]][i] of
+ * cos_table and sin_table [max_seq][rot_dim / 2]; in float32, each product and
+ * sum rounded on its own, the result rounded once to dtype.  inverse != 0
+ * rotates back (s negated; also the gradient of the rotation).  out may be x
+ * with the same strides, and may not overlap it in any other way.  A position
+ * outside [0, max_seq) leaves its token unwritten and vkq_device_status then
+ * reports VKQ_ERR_INVALID_ARGUMENT.  Element alignment suffices; 16-byte
+ * aligned rows and rot_dim a multiple of 16 take the vector path. */
+VKQ_API int vkq_rotary(int device, int dtype, const void *x, int64_t x_token_stride, int64_t x_head_stride, void *out,
+                       int64_t out_token_stride, int64_t out_head_stride, const float *cos_table,
+                       const float *sin_table, const int32_t *positions, int64_t tokens, int64_t heads,
+                       int64_t head_dim, int64_t rot_dim, int64_t max_seq, int layout, int inverse, void *stream);
+
+/* cos and sin tables [max_seq][rot_dim / 2] on the device: angle = position *
+ * f_i in float64, each entry rounded once.  With t_i = base^(-2i / rot_dim):
+ *   VKQ_ROPE_SCALE_NONE:   f_i = t_i
+ *   VKQ_ROPE_SCALE_LINEAR: f_i = t_i / factor (positions interpolated)
+ *   VKQ_ROPE_SCALE_NTK:    t_i with the base times factor^(rot_dim / (rot_dim - 2))
+ *   VKQ_ROPE_SCALE_YARN:   f_i = t_i / factor * w_i + t_i * (1 - w_i), w_i rising
+ *     from 0 to 1 between i = floor(d(beta_fast)) and ceil(d(beta_slow)),
+ *     d(b) = rot_dim * ln(orig_len / (2 pi b)) / (2 ln base): pairs that turn
+ *     often within orig_len stay, pairs that do not are interpolated; both
+ *     tables are multiplied by attn_factor (0: 0.1 ln(factor) + 1).
+ * factor >= 1; orig_len, beta_fast > beta_slow > 0 and attn_factor count for
+ * VKQ_ROPE_SCALE_YARN only. */
+#define VKQ_ROPE_SCALE_NONE 0
+#define VKQ_ROPE_SCALE_LINEAR 1
+#define VKQ_ROPE_SCALE_NTK 2
+#define VKQ_ROPE_SCALE_YARN 3
+VKQ_API int vkq_rotary_tables_f32(int device, float *cos_table, float *sin_table, int64_t max_seq, int64_t rot_dim,
+                                  double base, int scaling, double factor, int64_t orig_len, double beta_fast,
+                                  double beta_slow, double attn_factor, void *stream);
+
+/* The pool of an 8-bit paged KV cache, all layers.  A page holds page_size
+ * tokens of every KV head; VKQ_KV8_BLOCK tokens of a head share one positive
+ * scale for K and one for V: a value is its code times its scale.  Codes are
+ * two's complement int8 (-127..127) or e4m3 (no infinities, |x| <= 448).
+ * k, v: [layers][num_pages][kv_heads][page_size][head_dim] bytes, 16-byte
+ * aligned; k_scale, v_scale: [layers][num_pages][kv_heads][page_size / 16]
+ * float32.  head_dim 64 or 128; page_size a multiple of 16, at most 4096.
+ * vkq_kv8_append writes scales that are powers of two in [2^-64, 2^63]; the
+ * readers take any positive scale in that range. */
+#define VKQ_KV8_INT8 0
+#define VKQ_KV8_E4M3 1
+#define VKQ_KV8_BLOCK 16
+typedef struct vkq_kv8_cache {
+    int32_t format; /* VKQ_KV8_INT8 or VKQ_KV8_E4M3 */
+    int32_t page_size, kv_heads, head_dim;
+    int64_t layers, num_pages;
+    void *k, *v;
+    float *k_scale, *v_scale;
+} vkq_kv8_cache;
+
+/* The sequences that a call works on (device arrays).  Row r of `table` lists
+ * the pages of sequence r in order; lens[r] is its length in tokens, the new
+ * ones included.  Sequence b of the batch is row slots[b] (slots NULL: row b);
+ * its new tokens are rows cu_tokens[b] .. cu_tokens[b + 1] - 1 of q, k, v and
+ * out (cu_tokens NULL: row b alone) and stand at positions lens - n .. lens - 1.
+ * max_tokens bounds the new tokens of one sequence, max_len the lengths (the
+ * host's plan goes by them; the lengths themselves stay on the device, so a
+ * captured graph can be replayed while they grow).  A row, a length, a token
+ * range or a page outside its bounds makes no access: vkq_kv8_append leaves
+ * the sequence (or the block) out, vkq_kv8_attention gives NaN for the rows
+ * that it concerns, and vkq_device_status reports VKQ_ERR_INVALID_ARGUMENT. */
+typedef struct vkq_kv8_batch {
+    const int32_t *table;     /* [rows][max_pages] */
+    const int32_t *lens;      /* [rows] */
+    const int32_t *slots;     /* [batch] or NULL */
+    const int32_t *cu_tokens; /* [batch + 1] or NULL */
+    int64_t rows, max_pages, batch, tokens, max_tokens, max_len;
+} vkq_kv8_batch;
+
+/* Writes the new tokens' K and V ([tokens][kv_heads][head_dim] of dtype, the
+ * token at a stride of its own) into the pages of `layer`.  With tables
+ * (cos_table not NULL) K is rotated first at the token's position, as
+ * vkq_rotary does but without the rounding to dtype, and so is q (NULL: none)
+ * [tokens][heads][head_dim] into q_out (which may be q).  Every block of 16
+ * tokens and head is quantized by itself: with a the largest finite |x| of its
+ * new tokens and m = 127 or 448, s_new is the least power of two with
+ * a <= m * s_new (kept within [2^-64, 2^63]); a block that holds older tokens
+ * keeps its scale if that is larger, else its older codes are rounded again to
+ * s_new.  Codes are round-to-nearest-even of x / s, saturating; a NaN is
+ * stored as 0.  Blocks of no new token are not touched.  Element alignment
+ * suffices. */
+VKQ_API int vkq_kv8_append(int device, const vkq_kv8_cache *cache, int64_t layer, const vkq_kv8_batch *batch, int dtype,
+                           const void *k, int64_t k_token_stride, const void *v, int64_t v_token_stride,
+                           const void *q, int64_t q_token_stride, void *q_out, int64_t q_out_token_stride,
+                           int64_t heads, const float *cos_table, const float *sin_table, int64_t max_seq,
+                           int64_t rot_dim, int layout, void *stream);
+
+/* Reads rows back: k_out[i] and v_out[i] ([n][kv_heads][head_dim] of dtype,
+ * either may be NULL) are the cached K and V of sequence seq[i] of the batch at
+ * position pos[i].  A row outside gives NaN, and vkq_device_status reports it. */
+VKQ_API int vkq_kv8_read(int device, const vkq_kv8_cache *cache, int64_t layer, const vkq_kv8_batch *batch,
+                         const int32_t *seq, const int32_t *pos, int64_t n, int dtype, void *k_out, void *v_out,
+                         void *stream);
+
+/* Attention of the new tokens over the cache (which holds them already):
+ *   out[t][h] = sum_j p_j v_j,  p = softmax over the visible j of scale * (q[t][h] . k_j)
+ * with k, v of KV head h / (heads / kv_heads).  A token at position p sees
+ * j <= p (causal != 0) and, with window > 0 (causal only), j > p - window;
+ * causal == 0 sees every token of its sequence.  A token that sees none gives
+ * zeros.  q and out [tokens][heads][head_dim] of dtype, token strides of their
+ * own; heads a multiple of kv_heads; scale > 0.  Scores, softmax and sums are
+ * float32.  The codes are exact operands of the 16-bit matrix instructions;
+ * float32 q and probabilities go through them in two 11-bit parts (error
+ * within 1e-5 of sum_j p_j |v_j|, and what float32 scores carry: 2^-20 of
+ * scale sum_d |q_d k_jd|), 16-bit ones are rounded once to 11 bits; a p below
+ * 2^-39 of its row's largest adds nothing to the sum.  workspace: vkq_kv8_attention_workspace_bytes for these bounds,
+ * 16-byte aligned, zero-filled before its first use; every call leaves it
+ * ready for the next one.  Calls that may run at once need separate ones. */
+VKQ_API int vkq_kv8_attention_workspace_bytes(int device, const vkq_kv8_cache *cache, const vkq_kv8_batch *batch,
+                                              int dtype, int64_t heads, int causal, int64_t window, size_t *bytes);
+VKQ_API int vkq_kv8_attention(int device, const vkq_kv8_cache *cache, int64_t layer, const vkq_kv8_batch *batch,
+                              int dtype, const void *q, int64_t q_token_stride, void *out, int64_t out_token_stride,
+                              int64_t heads, float scale, int causal, int64_t window, void *workspace,
+                              size_t workspace_bytes, void *stream);
+
+/* The bookkeeping of a pool's pages (device arrays): table [rows][max_pages]
+ * (-1: no page), lens [rows], and refs [num_pages], how many rows hold the
+ * page (0: free).  An empty state is table -1, lens and refs 0.  Free pages
+ * are taken lowest number first.  The calls below work on the listed rows
+ * (distinct: a row listed again, or out of range, is left out and
+ * vkq_device_status reports VKQ_ERR_INVALID_ARGUMENT) and run on the device
+ * without a host read.  done (NULL: not wanted) receives 1 for a listed row
+ * that was served and 0 for one that was left as it was, because it is invalid
+ * or too few pages are free.  workspace: vkq_kv8_pages_workspace_bytes,
+ * 16-byte aligned, zero-filled before its first use, left ready by every call. */
+typedef struct vkq_kv8_seqs {
+    int32_t *table, *lens, *refs;
+    int64_t rows, max_pages;
+} vkq_kv8_seqs;
+VKQ_API int vkq_kv8_pages_workspace_bytes(const vkq_kv8_cache *cache, const vkq_kv8_seqs *seqs, size_t *bytes);
+/* Grows row slots[i] by add[i] >= 0 tokens: its length, and the pages that it
+ * then needs.  Pages go to the rows in the order listed; a row whose pages
+ * are past the last free one stays as it was. */
+VKQ_API int vkq_kv8_extend(int device, const vkq_kv8_cache *cache, const vkq_kv8_seqs *seqs, const int32_t *slots,
+                           const int32_t *add, int64_t n, int32_t *done, void *workspace, size_t workspace_bytes,
+                           void *stream);
+/* Makes the empty row dst[i] a copy of row src[i]: whole pages are shared, a
+ * part-filled last page is copied (all layers) into a free one, so that no
+ * append ever writes to a shared page. */
+VKQ_API int vkq_kv8_fork(int device, const vkq_kv8_cache *cache, const vkq_kv8_seqs *seqs, const int32_t *src,
+                         const int32_t *dst, int64_t n, int32_t *done, void *workspace, size_t workspace_bytes,
+                         void *stream);
+/* Empties the listed rows; a page that no row holds any more is free. */
+VKQ_API int vkq_kv8_free(int device, const vkq_kv8_cache *cache, const vkq_kv8_seqs *seqs, const int32_t *slots,
+                         int64_t n, int32_t *done, void *workspace, size_t workspace_bytes, void *stream);
+/* Moves pages down so that the U pages in use are pages 0 .. U - 1 (the k-th
+ * used page >= U goes to the k-th free page < U), all layers, and renames
+ * them in the table.  used (NULL: not wanted) receives U. */
+VKQ_API int vkq_kv8_compact(int device, const vkq_kv8_cache *cache, const vkq_kv8_seqs *seqs, int32_t *used,
+                            void *workspace, size_t workspace_bytes, void *stream);
+/* Copies the contents (codes and scales, all layers) of page src[i] to page
+ * dst[i]; no page may be both a source and a target, and targets are
+ * distinct.  A page out of range is left out and reported. */
+VKQ_API int vkq_kv8_copy_pages(int device, const vkq_kv8_cache *cache, const int32_t *src, const int32_t *dst,
+                               int64_t n, void *stream);
+
 /* Reads and clears the device-side status word of this library on a device
  * (set when a bounded wait inside a kernel gave up, or a peer was out of
  * step).  Synchronizes with the device.  *code receives VKQ_OK,

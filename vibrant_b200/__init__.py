@@ -5,7 +5,8 @@ include/vkq.h (built into vibrant_b200/_lib/libvkq.so).
 Modules:
   vkq      ctypes binding of the C ABI (what a cgo shim binds)
   tensor   torch-facing helpers over that binding (device buffers, streams)
+  kv8      an 8-bit paged KV cache: append, attention, page operations
   synth    seeded synthetic workloads
   build    nvcc build of libvkq.so
 """
-__all__ = ["vkq", "synth", "build"]
+__all__ = ["vkq", "kv8", "synth", "build"]

@@ -78,7 +78,7 @@ static int block_bytes(int qt) {
 
 // Makes the device current and checks it is a compute capability 10.x part
 // (the kernels are built for sm_100a only).
-static int enter(int device) {
+int enter(int device) {
     t_err[0] = '\0';
     int dev = device;
     int cur = -1;
@@ -109,7 +109,7 @@ static int enter(int device) {
     return VKQ_OK;
 }
 
-static int check_launch(cudaError_t e, const char *what) {
+int check_launch(cudaError_t e, const char *what) {
     if (e != cudaSuccess) {
         set_error("%s: %s", what, cudaGetErrorString(e));
         return VKQ_ERR_CUDA;
@@ -729,12 +729,21 @@ int vkq_device_status(int device, int *code) {
     const int g4 = gemv_strip_read_status();
     const int g5 = elem_read_status();
     const int g6 = attention_read_status();
+    const int g7 = rotary_read_status();
+    const int g8 = kv8_read_status();
+    const int g9 = kv8_attention_read_status();
+    const int g10 = kv8_pages_read_status();
     if (g == 0) g = g2;
     if (g == 0) g = g3;
     if (g == 0) g = g4;
     if (g == 0) g = g5;
     if (g == 0) g = g6;
-    if (g < 0 || g2 < 0 || g3 < 0 || g4 < 0 || g5 < 0 || g6 < 0) {
+    if (g == 0) g = g7;
+    if (g == 0) g = g8;
+    if (g == 0) g = g9;
+    if (g == 0) g = g10;
+    if (g < 0 || g2 < 0 || g3 < 0 || g4 < 0 || g5 < 0 || g6 < 0 || g7 < 0 || g8 < 0 || g9 < 0 ||
+        g10 < 0) {
         set_error("cannot read the device status word");
         return VKQ_ERR_CUDA;
     }

@@ -6,6 +6,8 @@
 #include <cstdint>
 #include <cuda_runtime.h>
 
+#include "../../include/vkq.h"
+
 namespace vkq {
 
 int device_sm_count(int device);
@@ -159,6 +161,76 @@ int elem_read_status();  // reads and clears the elementwise kernels' status wor
 // dst[0..n) = src[0..n) from pinned host memory through its device mapping
 // (elementwise.cu), as a kernel that takes part in programmatic dependent launch.
 cudaError_t stage_in(const float *src_mapped, float *dst, int64_t n, cudaStream_t s);
+
+// Rotary positions over strided activations and their tables (rotary.cu).
+struct RotaryArgs {
+    int dtype;
+    const void *x;
+    int64_t x_token, x_head;
+    void *out;
+    int64_t out_token, out_head;
+    const float *cos_t, *sin_t;
+    const int *positions;
+    int64_t tokens, heads, head_dim, rot_dim, max_seq;
+    int layout, inverse;
+};
+cudaError_t rotary(const RotaryArgs &a, cudaStream_t s, int device);
+cudaError_t rotary_tables(float *cos_t, float *sin_t, int64_t max_seq, int64_t rot_dim, double base, int scaling,
+                          double factor, int64_t orig_len, double beta_fast, double beta_slow, double attn_factor,
+                          cudaStream_t s, int device);
+int rotary_read_status();
+
+// The 8-bit paged KV cache: append and read-back (kv8_cache.cu), attention
+// (kv8_attention.cu), page operations (kv8_pages.cu).  Arguments are checked
+// by the entry points (kv8_api.cu).
+struct Kv8AppendArgs {
+    int dtype;
+    const void *k, *v, *q;
+    int64_t k_token, v_token, q_token;
+    void *q_out;
+    int64_t q_out_token, heads;
+    const float *cos_t, *sin_t;
+    int64_t max_seq, rot_dim;
+    int layout;
+};
+// Warps the append's launch needs (the grid's size).
+int64_t kv8_append_warps(const vkq_kv8_cache &c, const vkq_kv8_batch &b, int64_t heads, bool q);
+cudaError_t kv8_append(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_batch &b, const Kv8AppendArgs &a,
+                       cudaStream_t s);
+cudaError_t kv8_read(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_batch &b, const int *seq, const int *pos,
+                     int64_t n, int dtype, void *k_out, void *v_out, cudaStream_t s, int device);
+int kv8_read_status();
+struct Kv8AttentionArgs {
+    int dtype;
+    const void *q;
+    int64_t q_token;
+    void *out;
+    int64_t out_token, heads;
+    float scale;
+    int causal;
+    int64_t window;
+    void *workspace;
+};
+size_t kv8_attention_workspace(const vkq_kv8_cache &c, const vkq_kv8_batch &b, int dtype, int64_t heads, int causal,
+                               int64_t window, int device);
+cudaError_t kv8_attention(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_batch &b, const Kv8AttentionArgs &a,
+                          cudaStream_t s, int device);
+int kv8_attention_read_status();
+size_t kv8_pages_workspace(const vkq_kv8_cache &c, const vkq_kv8_seqs &q);
+cudaError_t kv8_extend(const vkq_kv8_cache &c, const vkq_kv8_seqs &q, const int *slots, const int *add, int64_t n,
+                       int *done, void *ws, cudaStream_t s);
+cudaError_t kv8_fork(const vkq_kv8_cache &c, const vkq_kv8_seqs &q, const int *src, const int *dst, int64_t n, int *done,
+                     void *ws, cudaStream_t s, int device);
+cudaError_t kv8_free(const vkq_kv8_cache &c, const vkq_kv8_seqs &q, const int *slots, int64_t n, int *done, void *ws,
+                     cudaStream_t s);
+cudaError_t kv8_compact(const vkq_kv8_cache &c, const vkq_kv8_seqs &q, int *used, void *ws, cudaStream_t s, int device);
+cudaError_t kv8_copy_pages(const vkq_kv8_cache &c, const int *src, const int *dst, int64_t n, cudaStream_t s, int device);
+int kv8_pages_read_status();
+
+// Makes `device` current and checks that the kernels can run on it; returns a
+// vkq_status code (capi.cu).  check_launch turns a CUDA error into one.
+int enter(int device);
+int check_launch(cudaError_t e, const char *what);
 
 void set_error(const char *fmt, ...);
 bool vkq_last_error_empty();

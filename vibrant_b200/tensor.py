@@ -126,6 +126,78 @@ def dequant_transpose(w: QuantWeight, stream=None) -> torch.Tensor:
     return out
 
 
+# ---- rotary positions ----
+
+DTYPE_CODES = {torch.float32: vkq.F32, torch.float16: vkq.F16, torch.bfloat16: vkq.BF16}
+ROPE_LAYOUTS = {"interleaved": vkq.ROPE_INTERLEAVED, "half": vkq.ROPE_HALF}
+ROPE_SCALINGS = {"none": vkq.ROPE_SCALE_NONE, "linear": vkq.ROPE_SCALE_LINEAR, "ntk": vkq.ROPE_SCALE_NTK,
+                 "yarn": vkq.ROPE_SCALE_YARN}
+
+
+def dtype_code(t: torch.Tensor) -> int:
+    try:
+        return DTYPE_CODES[t.dtype]
+    except KeyError:
+        raise ValueError(f"float32, float16 or bfloat16 needed, got {t.dtype}") from None
+
+
+def _device_index(t: torch.Tensor) -> int:
+    if not t.is_cuda:
+        raise ValueError("a CUDA tensor is needed")
+    return t.device.index
+
+
+def check_int32(t: torch.Tensor, shape: tuple, name: str, device: torch.device) -> None:
+    """An int32 contiguous tensor of that shape (None: any extent) on the device."""
+    if t.dtype != torch.int32 or t.device != device or not t.is_contiguous() or t.dim() != len(shape) or \
+            any(n is not None and n != m for n, m in zip(shape, t.shape)):
+        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {shape} on {device}, got "
+                         f"{tuple(t.shape)} {t.dtype} on {t.device}")
+
+
+def check_tables(cos: torch.Tensor, sin: torch.Tensor, device: torch.device) -> None:
+    if cos.dtype != torch.float32 or cos.dim() != 2 or cos.shape != sin.shape or sin.dtype != torch.float32 or \
+            not cos.is_contiguous() or not sin.is_contiguous() or cos.device != device or sin.device != device:
+        raise ValueError("cos and sin must be contiguous float32 tables [max_seq, rot_dim / 2] on the data's device")
+
+
+def rotary_tables(rot_dim: int, base: float, max_seq: int, scaling: str = "none", factor: float = 1.0,
+                  orig_len: int = 0, beta_fast: float = 32.0, beta_slow: float = 1.0, attn_factor: float = 0.0,
+                  device="cuda", stream: torch.cuda.Stream | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """cos and sin tables [max_seq, rot_dim / 2] built on the device
+    (vkq_rotary_tables_f32); scaling "none", "linear", "ntk" or "yarn"."""
+    cos = torch.empty((max_seq, rot_dim // 2), dtype=torch.float32, device=device)
+    sin = torch.empty_like(cos)
+    st = stream if stream is not None else torch.cuda.current_stream(cos.device)
+    vkq.rotary_tables_f32(cos.data_ptr(), sin.data_ptr(), max_seq, rot_dim, base, ROPE_SCALINGS[scaling], factor,
+                          orig_len, beta_fast, beta_slow, attn_factor, device=cos.device.index, stream=st)
+    return cos, sin
+
+
+def rotary(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor, layout: str = "interleaved",
+           inverse: bool = False, out: torch.Tensor | None = None,
+           stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    """Rotary positions of x [tokens, heads, head_dim] (any token and head
+    strides) by the tables' rows positions[t] (vkq_rotary); out may be x."""
+    if x.dim() != 3 or x.stride(2) != 1 and x.shape[2] > 1:
+        raise ValueError("x must be [tokens, heads, head_dim] with contiguous heads")
+    dev = _device_index(x)
+    check_tables(cos, sin, x.device)
+    check_int32(positions, (x.shape[0],), "positions", x.device)
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or out.stride(2) != 1:
+        raise ValueError("out must match x")
+    if x.numel() == 0:
+        return out
+    st = stream if stream is not None else torch.cuda.current_stream(x.device)
+    T, H, D = x.shape
+    vkq.rotary(dtype_code(x), x.data_ptr(), (x.stride(0), x.stride(1)), out.data_ptr(),
+               (out.stride(0), out.stride(1)), cos.data_ptr(), sin.data_ptr(), positions.data_ptr(), T, H, D,
+               2 * cos.shape[1], cos.shape[0], ROPE_LAYOUTS[layout], inverse, device=dev, stream=st)
+    return out
+
+
 # ---- row-sharded matmul across the GPUs of one node ----
 
 def shard_columns(N: int, world: int) -> tuple[int, list[tuple[int, int]]]:

@@ -24,6 +24,28 @@ _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
 _sz = ctypes.c_size_t
+
+
+class Kv8CacheStruct(ctypes.Structure):
+    """vkq_kv8_cache: the pool of an 8-bit paged KV cache."""
+    _fields_ = [("format", ctypes.c_int32), ("page_size", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("layers", _i64), ("num_pages", _i64), ("k", _vp), ("v", _vp),
+                ("k_scale", _vp), ("v_scale", _vp)]
+
+
+class Kv8BatchStruct(ctypes.Structure):
+    """vkq_kv8_batch: the sequences that a call works on."""
+    _fields_ = [("table", _vp), ("lens", _vp), ("slots", _vp), ("cu_tokens", _vp), ("rows", _i64),
+                ("max_pages", _i64), ("batch", _i64), ("tokens", _i64), ("max_tokens", _i64), ("max_len", _i64)]
+
+
+class Kv8SeqsStruct(ctypes.Structure):
+    """vkq_kv8_seqs: the bookkeeping of a pool's pages."""
+    _fields_ = [("table", _vp), ("lens", _vp), ("refs", _vp), ("rows", _i64), ("max_pages", _i64)]
+
+
+_cache_p, _batch_p, _seqs_p = (ctypes.POINTER(t) for t in (Kv8CacheStruct, Kv8BatchStruct, Kv8SeqsStruct))
+_f64 = ctypes.c_double
 SIGNATURES = {
     "vkq_abi_version": (_int, []),
     "vkq_status_string": (ctypes.c_char_p, [_int]),
@@ -60,6 +82,22 @@ SIGNATURES = {
                                               _i64, _i64, _i64, _i64, _vp]),
     "vkq_linear_fused": (_int, [_int, _int, _int, ctypes.POINTER(_vp), ctypes.POINTER(_i64), _i64,
                                 ctypes.POINTER(_i64), _vp, _i64, _vp, ctypes.c_float, _int, ctypes.POINTER(_vp), _vp]),
+    "vkq_rotary": (_int, [_int, _int, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
+                          _int, _int, _vp]),
+    "vkq_rotary_tables_f32": (_int, [_int, _vp, _vp, _i64, _i64, _f64, _int, _f64, _i64, _f64, _f64, _f64, _vp]),
+    "vkq_kv8_append": (_int, [_int, _cache_p, _i64, _batch_p, _int, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64,
+                              _vp, _vp, _i64, _i64, _int, _vp]),
+    "vkq_kv8_read": (_int, [_int, _cache_p, _i64, _batch_p, _vp, _vp, _i64, _int, _vp, _vp, _vp]),
+    "vkq_kv8_attention_workspace_bytes": (_int, [_int, _cache_p, _batch_p, _int, _i64, _int, _i64,
+                                                 ctypes.POINTER(_sz)]),
+    "vkq_kv8_attention": (_int, [_int, _cache_p, _i64, _batch_p, _int, _vp, _i64, _vp, _i64, _i64, ctypes.c_float,
+                                 _int, _i64, _vp, _sz, _vp]),
+    "vkq_kv8_pages_workspace_bytes": (_int, [_cache_p, _seqs_p, ctypes.POINTER(_sz)]),
+    "vkq_kv8_extend": (_int, [_int, _cache_p, _seqs_p, _vp, _vp, _i64, _vp, _vp, _sz, _vp]),
+    "vkq_kv8_fork": (_int, [_int, _cache_p, _seqs_p, _vp, _vp, _i64, _vp, _vp, _sz, _vp]),
+    "vkq_kv8_free": (_int, [_int, _cache_p, _seqs_p, _vp, _i64, _vp, _vp, _sz, _vp]),
+    "vkq_kv8_compact": (_int, [_int, _cache_p, _seqs_p, _vp, _vp, _sz, _vp]),
+    "vkq_kv8_copy_pages": (_int, [_int, _cache_p, _vp, _vp, _i64, _vp]),
     "vkq_gguf_open": (_int, [ctypes.c_char_p, ctypes.POINTER(_vp)]),
     "vkq_gguf_close": (_int, [_vp]),
     "vkq_gguf_tensor_count": (_i64, [_vp]),
@@ -249,6 +287,107 @@ def rope_tables(head_dim: int, freq_base: float, max_seq: int):
     freq = 1.0 / np.power(freq_base, 2.0 * i / head_dim)
     angle = np.arange(max_seq, dtype=np.float64)[:, None] * freq[None, :]
     return np.cos(angle).astype(np.float32), np.sin(angle).astype(np.float32)
+
+
+# ---- serving: rotary positions and the 8-bit paged KV cache ----
+
+F32, F16, BF16 = 0, 1, 30  # element types of activations
+ROPE_INTERLEAVED, ROPE_HALF = 0, 1
+ROPE_SCALE_NONE, ROPE_SCALE_LINEAR, ROPE_SCALE_NTK, ROPE_SCALE_YARN = range(4)
+KV8_INT8, KV8_E4M3 = 0, 1
+KV8_BLOCK = 16
+
+
+def rotary(dtype: int, x_ptr: int, x_strides: tuple[int, int], out_ptr: int, out_strides: tuple[int, int],
+           cos_ptr: int, sin_ptr: int, pos_ptr: int, tokens: int, heads: int, head_dim: int, rot_dim: int,
+           max_seq: int, layout: int, inverse: bool = False, device: int = -1, stream=None) -> None:
+    """vkq_rotary: rotary positions over [tokens][heads][head_dim] at the
+    given (token, head) strides, in elements."""
+    _check(load().vkq_rotary(device, dtype, x_ptr, x_strides[0], x_strides[1], out_ptr, out_strides[0],
+                             out_strides[1], cos_ptr, sin_ptr, pos_ptr, tokens, heads, head_dim, rot_dim, max_seq,
+                             layout, int(inverse), _stream_ptr(stream)))
+
+
+def rotary_tables_f32(cos_ptr: int, sin_ptr: int, max_seq: int, rot_dim: int, base: float,
+                      scaling: int = ROPE_SCALE_NONE, factor: float = 1.0, orig_len: int = 0, beta_fast: float = 32.0,
+                      beta_slow: float = 1.0, attn_factor: float = 0.0, device: int = -1, stream=None) -> None:
+    """vkq_rotary_tables_f32: cos and sin tables [max_seq][rot_dim / 2]."""
+    _check(load().vkq_rotary_tables_f32(device, cos_ptr, sin_ptr, max_seq, rot_dim, base, scaling, factor, orig_len,
+                                        beta_fast, beta_slow, attn_factor, _stream_ptr(stream)))
+
+
+def kv8_append(cache: Kv8CacheStruct, layer: int, batch: Kv8BatchStruct, dtype: int, k_ptr: int, k_stride: int,
+               v_ptr: int, v_stride: int, q_ptr: int | None = None, q_stride: int = 0, q_out_ptr: int | None = None,
+               q_out_stride: int = 0, heads: int = 0, cos_ptr: int | None = None, sin_ptr: int | None = None,
+               max_seq: int = 0, rot_dim: int = 0, layout: int = ROPE_INTERLEAVED, device: int = -1,
+               stream=None) -> None:
+    """vkq_kv8_append: the new tokens' K (rotated) and V into the cache, q rotated beside."""
+    _check(load().vkq_kv8_append(device, ctypes.byref(cache), layer, ctypes.byref(batch), dtype, k_ptr, k_stride,
+                                 v_ptr, v_stride, q_ptr, q_stride, q_out_ptr, q_out_stride, heads, cos_ptr, sin_ptr,
+                                 max_seq, rot_dim, layout, _stream_ptr(stream)))
+
+
+def kv8_read(cache: Kv8CacheStruct, layer: int, batch: Kv8BatchStruct, seq_ptr: int, pos_ptr: int, n: int, dtype: int,
+             k_ptr: int | None, v_ptr: int | None, device: int = -1, stream=None) -> None:
+    """vkq_kv8_read: cached rows (sequence, position) as values."""
+    _check(load().vkq_kv8_read(device, ctypes.byref(cache), layer, ctypes.byref(batch), seq_ptr, pos_ptr, n, dtype,
+                               k_ptr, v_ptr, _stream_ptr(stream)))
+
+
+def kv8_attention_workspace_bytes(cache: Kv8CacheStruct, batch: Kv8BatchStruct, dtype: int, heads: int,
+                                  causal: bool = True, window: int = 0, device: int = -1) -> int:
+    out = _sz()
+    _check(load().vkq_kv8_attention_workspace_bytes(device, ctypes.byref(cache), ctypes.byref(batch), dtype, heads,
+                                                    int(causal), window, ctypes.byref(out)))
+    return out.value
+
+
+def kv8_attention(cache: Kv8CacheStruct, layer: int, batch: Kv8BatchStruct, dtype: int, q_ptr: int, q_stride: int,
+                  out_ptr: int, out_stride: int, heads: int, scale: float, ws_ptr: int | None, ws_bytes: int,
+                  causal: bool = True, window: int = 0, device: int = -1, stream=None) -> None:
+    """vkq_kv8_attention: the new tokens' attention over the cache."""
+    _check(load().vkq_kv8_attention(device, ctypes.byref(cache), layer, ctypes.byref(batch), dtype, q_ptr, q_stride,
+                                    out_ptr, out_stride, heads, scale, int(causal), window, ws_ptr, ws_bytes,
+                                    _stream_ptr(stream)))
+
+
+def kv8_pages_workspace_bytes(cache: Kv8CacheStruct, seqs: Kv8SeqsStruct) -> int:
+    out = _sz()
+    _check(load().vkq_kv8_pages_workspace_bytes(ctypes.byref(cache), ctypes.byref(seqs), ctypes.byref(out)))
+    return out.value
+
+
+def kv8_extend(cache: Kv8CacheStruct, seqs: Kv8SeqsStruct, slots_ptr: int, add_ptr: int, n: int, done_ptr: int | None,
+               ws_ptr: int, ws_bytes: int, device: int = -1, stream=None) -> None:
+    """vkq_kv8_extend: lengths and pages of the listed rows grow."""
+    _check(load().vkq_kv8_extend(device, ctypes.byref(cache), ctypes.byref(seqs), slots_ptr, add_ptr, n, done_ptr,
+                                 ws_ptr, ws_bytes, _stream_ptr(stream)))
+
+
+def kv8_fork(cache: Kv8CacheStruct, seqs: Kv8SeqsStruct, src_ptr: int, dst_ptr: int, n: int, done_ptr: int | None,
+             ws_ptr: int, ws_bytes: int, device: int = -1, stream=None) -> None:
+    """vkq_kv8_fork: the empty rows dst become copies of the rows src."""
+    _check(load().vkq_kv8_fork(device, ctypes.byref(cache), ctypes.byref(seqs), src_ptr, dst_ptr, n, done_ptr, ws_ptr,
+                               ws_bytes, _stream_ptr(stream)))
+
+
+def kv8_free(cache: Kv8CacheStruct, seqs: Kv8SeqsStruct, slots_ptr: int, n: int, done_ptr: int | None, ws_ptr: int,
+             ws_bytes: int, device: int = -1, stream=None) -> None:
+    """vkq_kv8_free: the listed rows become empty."""
+    _check(load().vkq_kv8_free(device, ctypes.byref(cache), ctypes.byref(seqs), slots_ptr, n, done_ptr, ws_ptr,
+                               ws_bytes, _stream_ptr(stream)))
+
+
+def kv8_compact(cache: Kv8CacheStruct, seqs: Kv8SeqsStruct, used_ptr: int | None, ws_ptr: int, ws_bytes: int,
+                device: int = -1, stream=None) -> None:
+    """vkq_kv8_compact: the pages in use become the lowest ones."""
+    _check(load().vkq_kv8_compact(device, ctypes.byref(cache), ctypes.byref(seqs), used_ptr, ws_ptr, ws_bytes,
+                                  _stream_ptr(stream)))
+
+
+def kv8_copy_pages(cache: Kv8CacheStruct, src_ptr: int, dst_ptr: int, n: int, device: int = -1, stream=None) -> None:
+    """vkq_kv8_copy_pages: the contents of pages src become those of pages dst."""
+    _check(load().vkq_kv8_copy_pages(device, ctypes.byref(cache), src_ptr, dst_ptr, n, _stream_ptr(stream)))
 
 
 def device_status(device: int = -1) -> int:
