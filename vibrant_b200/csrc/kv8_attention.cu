@@ -47,7 +47,6 @@ constexpr int kDecWarps = 4;
 constexpr int kDecThreads = 32 * kDecWarps;
 constexpr int kDecStep = 32;   // keys of a step: two scale blocks
 constexpr int kDecStages = 3;  // ring slots of a warp: two steps in flight
-constexpr uint32_t kHeadCounters = (uint32_t)(kWorkspaceCounterHead / sizeof(unsigned));
 
 struct DecodeParams {
     Kv8Pool pool;
@@ -169,7 +168,7 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const DecodePar
         }
         a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
         a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
-        const int e = min(max((int)(__float_as_uint(a) >> 23) - 127, -100), 127);
+        const int e = min(max((int)(__float_as_uint(a) >> 23) - 127, -60), 127);
         const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
         rf[u] = p.f * __uint_as_float((uint32_t)(e - 14 + 127) << 23) * (E4M3 ? 256.f : 1.f);
 #pragma unroll
@@ -462,16 +461,9 @@ static const void *decode_fn(int D, bool e4m3) {
     return D == 64 ? decode_fn<T, 64>(e4m3) : decode_fn<T, 128>(e4m3);
 }
 
-// How a call is cut: tiles of rows, ranges of keys.
-struct DecodePlan {
-    int rows, row_tiles, splits, chunk;
-    int64_t tiles;
-    size_t part_floats, stat_floats;
-};
-
-static DecodePlan decode_plan(const vkq_kv8_cache &c, const vkq_kv8_batch &b, int dtype, int64_t heads, int causal,
+static Kv8Plan decode_plan(const vkq_kv8_cache &c, const vkq_kv8_batch &b, int dtype, int64_t heads, int causal,
                               int64_t window, int sms) {
-    DecodePlan q{};
+    Kv8Plan q{};
     q.rows = dtype == VKQ_F32 ? 8 : 16;
     const int64_t g = heads / c.kv_heads;
     q.row_tiles = (int)((b.max_tokens * g + q.rows - 1) / q.rows);
@@ -503,15 +495,28 @@ static DecodePlan decode_plan(const vkq_kv8_cache &c, const vkq_kv8_batch &b, in
     return q;
 }
 
+// Rows of a sequence and KV head from which the 128-row tiles pay.
+static bool many_rows(const vkq_kv8_cache &c, const vkq_kv8_batch &b, int64_t heads) {
+    return b.max_tokens * (heads / c.kv_heads) > 64;
+}
+
+static Kv8Plan attention_plan(const vkq_kv8_cache &c, const vkq_kv8_batch &b, int dtype, int64_t heads, int causal,
+                              int64_t window, int device) {
+    const int sms = device_sm_count(device);
+    return many_rows(c, b, heads) ? kv8_prefill_plan(c, b, dtype, heads, causal, window, sms)
+                                  : decode_plan(c, b, dtype, heads, causal, window, sms);
+}
+
 size_t kv8_attention_workspace(const vkq_kv8_cache &c, const vkq_kv8_batch &b, int dtype, int64_t heads, int causal,
                                int64_t window, int device) {
-    const DecodePlan q = decode_plan(c, b, dtype, heads, causal, window, device_sm_count(device));
+    const Kv8Plan q = attention_plan(c, b, dtype, heads, causal, window, device);
     return kWorkspaceCounterHead + (q.part_floats + q.stat_floats) * sizeof(float);
 }
 
 cudaError_t kv8_attention(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_batch &b, const Kv8AttentionArgs &a,
                           cudaStream_t s, int device) {
-    const DecodePlan q = decode_plan(c, b, a.dtype, a.heads, a.causal, a.window, device_sm_count(device));
+    const Kv8Plan q = attention_plan(c, b, a.dtype, a.heads, a.causal, a.window, device);
+    if (many_rows(c, b, a.heads)) return kv8_prefill(c, layer, b, a, q, s);
     DecodeParams p{};
     p.pool = kv8_pool(c, layer);
     p.batch = kv8_batch(b);
@@ -551,7 +556,8 @@ int kv8_attention_read_status() {
     int v = 0, zero = 0;
     if (cudaMemcpyFromSymbol(&v, g_kv8_attn_status, sizeof(int)) != cudaSuccess) return -1;
     cudaMemcpyToSymbol(g_kv8_attn_status, &zero, sizeof(int));
-    return v;
+    const int w = kv8_prefill_read_status();
+    return w < 0 || v == 0 ? w : v;
 }
 
 }  // namespace vkq

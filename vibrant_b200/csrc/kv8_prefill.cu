@@ -1,0 +1,845 @@
+// kv8_prefill.cu -- attention of many query rows (chunks of prompts) over the
+// 8-bit paged KV cache, on tcgen05 with TMEM.
+//
+// The rows of a tile are (new token, query head) pairs of one sequence and KV
+// head, as in kv8_attention.cu, so the heads of a group share every key tile.
+// A CTA (one per SM, four warpgroups) takes one tile of rows and a range of
+// keys in tiles of 128:
+//   warpgroup 2 turns the pages' codes into float16 K and V tiles in shared
+//     memory (exact; 128-byte swizzle, one layout read K-major as K and
+//     MN-major as V), a ring of four;
+//   one warp of warpgroup 3 issues the products;
+//   warpgroups 0 and 1 work on the scores, a thread a row.
+// The block scales never touch the operands.  With x = f ks (q . ck) the
+// score of a key in units of log2 and lv = log2 vs,
+//   e = exp2(x + lv - M),  M the running maximum of x + lv,
+//   O = sum e cv,  l = sum e / vs,  o = O / l:
+// vs goes into the exponent, so that the second product's operand stays
+// within (0, 1], and out of the sum.  Both scales of 16 keys cost a thread two
+// multiplications a tile.
+//
+// 16-bit q: 256 rows, two halves of 128 in turn: while the scores of one half
+// are worked on, the products of the other run, and a K or V tile is converted
+// once for 256 rows.  e is rounded to 11 bits; the output stays in TMEM, and M
+// is raised (and the output rescaled) only when the maximum grew by more than
+// 2^8, which the operand's range allows.
+// float32 q: 128 rows; q and e are split into two 11-bit parts, so a tile
+// takes the same four products.  The matrix unit's accumulators round toward
+// zero, which would add up over a long cache: every key tile's output starts
+// from zero, and warpgroup 1 adds it to float32 registers while warpgroup 0
+// works on the next scores.
+//
+// Row tiles go from the last (which sees most keys) to the first, so that the
+// longest start first.  Few tiles are split along the keys, and joined in
+// order by the CTA that finishes last.
+#include <atomic>
+#include <cmath>
+#include <cstdint>
+
+#include "../../include/vkq.h"
+#include "act.cuh"
+#include "kq_device.cuh"
+#include "kv8.cuh"
+#include "umma.cuh"
+#include "vkq_internal.h"
+
+namespace vkq {
+
+static __device__ int g_kv8_prefill_status;
+
+constexpr int kPreThreads = 512;
+constexpr int kPreKeys = 128;                    // keys of a tile
+constexpr int kPreBlocks = kPreKeys / kKv8Block;  // and its scale blocks
+constexpr int kPreRing = 4;
+constexpr uint64_t kPreWaitNs = 2000000000ull;
+// registers a thread of warpgroups 0 and 1, of 2, of 3: at most 4 x 128 in all
+constexpr int kRegScore = 184, kRegConvert = 104, kRegIssue = 40;
+
+struct PrefillParams {
+    Kv8Pool pool;
+    Kv8Batch batch;
+    const void *q;
+    void *out;
+    int64_t qt, ot;
+    int heads, g, row_tiles, splits, chunk;
+    float f;  // scale * log2(e)
+    int causal, window;
+    bool vec;
+    float *part, *stat;
+    unsigned *count;
+};
+
+__device__ __forceinline__ void umma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+// The first operand in TMEM: a row a lane, two float16 a column.
+__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+// float16 operands, float32 accumulation, 128 rows; vn: the second operand N-major.
+__host__ __device__ constexpr uint32_t idesc_f16(int n, bool vn) {
+    return (1u << 4) | ((vn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+// 32 consecutive TMEM columns of the thread's lane; the caller waits (tmem_wait_ld) before using them.
+__device__ __forceinline__ void tmem_ld32(uint32_t (&r)[32], uint32_t addr) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+        "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, "
+        "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
+          "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
+          "=r"(r[30]), "=r"(r[31])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {"
+        "%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, "
+        "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+        ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
+        "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
+        "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+// Waits for the thread's TMEM loads; r passes through, so that no use of it moves above the wait.
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                 "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
+                 "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
+                 "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 ::"memory");
+}
+// The same with eight and sixteen columns.
+__device__ __forceinline__ void tmem_ld8(uint32_t (&r)[8], uint32_t addr) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[8]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]),
+                   "+r"(r[5]), "+r"(r[6]), "+r"(r[7])
+                 ::"memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                 ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+__device__ __forceinline__ float ex2p(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ float2 unpack_half(uint32_t b) { return __half22float2(*reinterpret_cast<const __half2 *>(&b)); }
+__device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
+// 16 codes as 16 float16 (the conversions of kv8_attention.cu).
+template <bool E4M3>
+__device__ __forceinline__ void codes_to_half(const uint4 &raw, uint32_t (&h)[8]) {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (E4M3) {
+            const uint32_t a = prmt(w[i], 0u, 0x1404u), b = prmt(w[i], 0u, 0x3424u);
+            h[2 * i] = (a & 0x80008000u) | ((a >> 1) & 0x3F803F80u);
+            h[2 * i + 1] = (b & 0x80008000u) | ((b >> 1) & 0x3F803F80u);
+        } else {
+            const uint32_t u = w[i] ^ 0x80808080u;
+            const uint32_t a = prmt(u, 0x64646464u, 0x4140u), b = prmt(u, 0x64646464u, 0x4342u);
+            const __half2 off = __half2half2(__ushort_as_half(0x6480));
+            const __half2 x = __hsub2(*reinterpret_cast<const __half2 *>(&a), off);
+            const __half2 y = __hsub2(*reinterpret_cast<const __half2 *>(&b), off);
+            h[2 * i] = *reinterpret_cast<const uint32_t *>(&x);
+            h[2 * i + 1] = *reinterpret_cast<const uint32_t *>(&y);
+        }
+    }
+}
+
+// Byte offset of 16-byte piece pc (of D / 8) of row r in a float16 tile of
+// 128 rows: halves of 64 values, 128-byte rows, pieces swizzled by the row.
+__device__ __forceinline__ uint32_t tile_off(int r, int pc) {
+    return (uint32_t)((pc >> 3) * (kPreKeys * 128) + r * 128 + (((pc & 7) ^ (r & 7)) << 4));
+}
+
+template <typename T, int D, bool E4M3>
+__global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const PrefillParams p) {
+    constexpr bool SPLIT = sizeof(T) == 4;
+    constexpr int ROWS = SPLIT ? 128 : 256;
+    constexpr uint32_t TILE = 128 * D * 2;          // bytes of a float16 tile of 128 rows
+    constexpr uint32_t HALF = kPreKeys * 128;       // its second half of 64 values
+    constexpr float kUp = SPLIT ? 14.f : 6.f;       // e is held as 2^kUp e (at most 2^14)
+    constexpr float kOut = E4M3 ? 256.f : 1.f;      // e4m3 operands are 2^8 too small
+    // TMEM columns: the scores (and, over them, e) of half or parity 0 and 1, the outputs
+    constexpr uint32_t kS = 0, kO = 256;
+    extern __shared__ __align__(1024) uint8_t smem[];  // two q tiles, the ring
+    __shared__ __align__(8) uint64_t bars[2 * kPreRing + 2 + 2 + 2 + 2 + 1];
+    __shared__ __align__(16) float scales[4][3][kPreBlocks];  // of key tile j & 3: ks, lv, 1 / vs
+    __shared__ float alpha[4][128], lsum[128], msum[128];
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile uint32_t abort_flag;
+    __shared__ uint32_t bad_flag;
+    __shared__ bool last;
+    pdl_wait();
+    pdl_launch_dependents();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = warp >> 2, t = tid & 127;
+    // block = ((reversed row tile, range), sequence, KV head), the last fastest
+    const int kvh = (int)(blockIdx.x % p.pool.kv_heads), x0 = (int)(blockIdx.x / p.pool.kv_heads);
+    const int seq = x0 % (int)p.batch.batch, x1 = x0 / (int)p.batch.batch;
+    const int rt = p.row_tiles - 1 - x1 / p.splits, split = x1 % p.splits;
+    const Kv8Seq s = kv8_seq(p.batch, p.pool.page, seq);
+    const int rows_all = s.n * p.g;
+    const int r0 = rt * ROWS;
+    if (!s.ok) {
+        if (split > 0) return;
+        if (tid == 0) atomicExch(&g_kv8_prefill_status, VKQ_ERR_INVALID_ARGUMENT);
+        for (int64_t i = tid; i < (int64_t)ROWS * D; i += kPreThreads) {
+            const int r = r0 + (int)(i / D);
+            if (r < rows_all)
+                static_cast<T *>(p.out)[(int64_t)(s.first + r / p.g) * p.ot + (int64_t)(kvh * p.g + r % p.g) * D + i % D] =
+                    from_f32<T>(__int_as_float(0x7fc00000));
+        }
+        return;
+    }
+    if (r0 >= rows_all) return;
+    const int pos0 = s.len - s.n;
+    const int row_end = min(r0 + ROWS, rows_all) - 1;
+    const int hi = p.causal ? max(pos0 + row_end / p.g + 1, 0) : s.len;
+    int lo = 0;
+    if (p.window > 0) lo = max(pos0 + r0 / p.g - p.window + 1, 0) & ~(kKv8Block - 1);
+    const int active = max((hi - lo + p.chunk - 1) / p.chunk, 1);
+    if (split >= active) return;
+    const int k_lo = lo + split * p.chunk, k_hi = min(hi, k_lo + p.chunk);
+    const int n = k_hi > k_lo ? (k_hi - k_lo + kPreKeys - 1) / kPreKeys : 0;  // key tiles
+    const bool two = !SPLIT && rows_all - r0 > 128;  // the second half has rows
+
+    const uint32_t base = (smem_u32addr(smem) + 1023u) & ~1023u;
+    const uint32_t q_tile = base, ring = base + 2 * TILE;
+    auto bar = [&](int i) { return smem_u32addr(&bars[i]); };
+    constexpr int FULL = 0, EMPTY = kPreRing, SF = 2 * kPreRing, PF = SF + 2, TF = PF + 2, TE = TF + 2, DR = TE + 2;
+    if (tid == 0) {
+        for (int i = 0; i < kPreRing; i++) {
+            mbar_init(bar(FULL + i), 4);   // a lane of each converting warp
+            mbar_init(bar(EMPTY + i), 1);  // commit
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(bar(SF + i), 1);  // commit: scores
+            mbar_init(bar(PF + i), 4);  // e is in TMEM
+            mbar_init(bar(TF + i), 1);  // commit: output (SPLIT: of one key tile)
+            mbar_init(bar(TE + i), 4);  // SPLIT: it has been read
+        }
+        mbar_init(bar(DR), 1);
+        mbar_init_fence();
+        abort_flag = 0;
+        bad_flag = 0;
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32addr(&tmem_slot)));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    // q: thread t of warpgroup 0 (and 1: the second half) loads its row, scales
+    // it below 2^15 by a power of two and stores its float16 tile (SPLIT: both
+    // parts, warpgroup 0)
+    float rf = 0.f;
+    int see_lo = 0, see_hi = 0;
+    if (wg == 0 || (wg == 1 && !SPLIT)) {
+        const int r = r0 + 128 * wg + t;
+        const bool there = r < rows_all;
+        const int i = there ? r / p.g : 0, h = kvh * p.g + (there ? r % p.g : 0);
+        const int ps = pos0 + i;
+        see_hi = !there ? 0 : min(p.causal ? ps + 1 : s.len, k_hi);
+        see_lo = p.window > 0 ? ps - p.window + 1 : 0;
+        const T *q = static_cast<const T *>(p.q) + (int64_t)(s.first + i) * p.qt + (int64_t)h * D;
+        float a = 0.f;
+        for (int c = 0; c < D; c += 8) {
+            float x[8];
+            load_act<T, 8>(q + c, x, p.vec);
+#pragma unroll
+            for (int u = 0; u < 8; u++) a = fmaxf(a, fabsf(x[u]));
+        }
+        const int e = min(max((int)(__float_as_uint(a) >> 23) - 127, -60), 127);
+        const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
+        rf = p.f * __uint_as_float((uint32_t)(e - 14 + 127) << 23) * kOut;
+        const uint32_t dst = q_tile + (SPLIT ? 0u : (uint32_t)wg * TILE);
+        for (int c = 0; c < D; c += 8) {
+            float x[8];
+            load_act<T, 8>(q + c, x, p.vec);
+            uint32_t b[4], b2[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const float x0 = x[2 * u] * up, x1 = x[2 * u + 1] * up;
+                b[u] = pack_half(x0, x1);
+                if constexpr (SPLIT) {
+                    const float2 back = unpack_half(b[u]);
+                    b2[u] = pack_half(x0 - back.x, x1 - back.y);
+                }
+            }
+            sts128(dst + tile_off(t, c / 8), b[0], b[1], b[2], b[3]);
+            if constexpr (SPLIT) sts128(dst + TILE + tile_off(t, c / 8), b2[0], b2[1], b2[2], b2[3]);
+        }
+        fence_async();
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = tmem_slot;
+
+    auto wait = [&](uint32_t b, uint32_t parity) -> bool {
+        if (mbar_wait_spin(b, parity, kPreWaitNs)) return true;
+        atomicExch(&g_kv8_prefill_status, kStatusTimeout);
+        abort_flag = 1;
+        return false;
+    };
+    // for whole warps: no lane goes on alone
+    auto wait_warp = [&](uint32_t b, uint32_t parity) -> bool { return __all_sync(0xffffffffu, wait(b, parity)); };
+    auto arrive = [&](uint32_t b) {  // once for the warp, after all its lanes
+        __syncwarp();
+        if (lane == 0) mbar_arrive(b);
+    };
+
+    const int64_t tile = ((int64_t)seq * p.pool.kv_heads + kvh) * p.row_tiles + rt;
+    // The ring's tiles in the order in which the products take them:
+    // K0, then V(j), K(j + 1) (SPLIT: K(j + 1), V(j): the scores of a tile are
+    // asked for before the output of the one before).
+    if (wg == 2) {
+        // ---- codes to float16 tiles ----
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegConvert));
+        constexpr int PER = kPreKeys * D / 16 / 128;  // 16-byte pieces of a tile that a thread takes: 8 or 4
+        constexpr int CPR = D / 16;                   // pieces of a row
+        constexpr int RSTEP = 128 / CPR;              // rows between a thread's pieces: 16 or 32
+        const int row0 = t / CPR, ch = t % CPR;
+        const int per_page = p.pool.page / kKv8Block;
+        auto load = [&](int j, bool is_v, uint4 (&raw)[PER]) {
+            const uint8_t *codes = is_v ? p.pool.v : p.pool.k;
+#pragma unroll
+            for (int k = 0; k < PER; k++) {
+                const int row = row0 + k * RSTEP, key = k_lo + j * kPreKeys + row;
+                raw[k] = make_uint4(0, 0, 0, 0);
+                if (key < k_hi) {
+                    const int blk = key / kKv8Block, lp = blk / per_page;
+                    const int id = kv8_page(p.pool, s, lp);
+                    if (id < 0) {
+                        bad_flag = 1;
+                    } else {
+                        const int64_t r = ((int64_t)id * p.pool.kv_heads + kvh) * p.pool.page + (key - lp * p.pool.page);
+                        raw[k] = *reinterpret_cast<const uint4 *>(codes + r * D + ch * 16);
+                    }
+                }
+            }
+        };
+        auto load_scales = [&](int j, float &ks, float &vs) {  // threads 0 .. 7
+            ks = vs = 1.f;
+            const int key = k_lo + j * kPreKeys + t * kKv8Block;
+            if (t < kPreBlocks && key < k_hi) {
+                const int blk = key / kKv8Block, lp = blk / per_page;
+                const int id = kv8_page(p.pool, s, lp);
+                if (id >= 0) {
+                    const int64_t e = ((int64_t)id * p.pool.kv_heads + kvh) * per_page + (blk - lp * per_page);
+                    ks = p.pool.ks[e];
+                    vs = p.pool.vs[e];
+                }
+            }
+        };
+        uint4 raw[PER], next[PER];
+        float ks, vs, ks_n = 1.f, vs_n = 1.f;
+        int j = 0;
+        bool is_v = false;
+        if (n > 0) {
+            load(0, false, raw);
+            load_scales(0, ks, vs);
+        }
+        int k_done = 0, v_done = 0;  // tiles handed over
+        RingPos rp;
+        for (int it = 0; it < 2 * n; it++) {
+            // the tile after this one
+            int kd = k_done + !is_v, vd = v_done + is_v;
+            bool nv;
+            if (SPLIT) nv = !(kd < n && kd < vd + 2);
+            else nv = vd < kd;
+            const int nj = nv ? vd : kd;
+            if (it + 1 < 2 * n) {
+                load(nj, nv, next);
+                if (!nv) load_scales(nj, ks_n, vs_n);
+            }
+            if (rp.uses >= (uint32_t)kPreRing && !wait_warp(bar(EMPTY + rp.idx), rp.phase ^ 1u)) break;
+            const uint32_t dst = ring + rp.idx * TILE;
+#pragma unroll
+            for (int k = 0; k < PER; k++) {
+                uint32_t h[8];
+                codes_to_half<E4M3>(raw[k], h);
+                const int row = row0 + k * RSTEP;
+                const uint32_t a = dst + tile_off(row, 2 * ch), b = dst + tile_off(row, 2 * ch + 1);
+                // eight lanes of one row: pieces of both halves fall into different banks
+                const bool odd = ch >= 4;
+                sts128(odd ? b : a, odd ? h[4] : h[0], odd ? h[5] : h[1], odd ? h[6] : h[2], odd ? h[7] : h[3]);
+                sts128(odd ? a : b, odd ? h[0] : h[4], odd ? h[1] : h[5], odd ? h[2] : h[6], odd ? h[3] : h[7]);
+            }
+            if (!is_v && t < kPreBlocks) {
+                scales[j & 3][0][t] = ks;
+                scales[j & 3][1][t] = __log2f(vs);
+                scales[j & 3][2][t] = 1.f / vs;
+            }
+            fence_async();
+            arrive(bar(FULL + rp.idx));
+            rp.next(kPreRing);
+            k_done = kd, v_done = vd;
+            j = nj, is_v = nv;
+#pragma unroll
+            for (int k = 0; k < PER; k++) raw[k] = next[k];
+            if (!nv) ks = ks_n, vs = vs_n;
+        }
+    } else if (wg == 3) {
+        // ---- the products ----
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegIssue));
+        if (warp == 12 && lane == 0 && n > 0) {
+            constexpr uint32_t IQK = idesc_f16(kPreKeys, false), IPV = idesc_f16(D, true);
+            RingPos rp;
+            bool ok = true;
+            auto take = [&](uint32_t &slot) {
+                slot = rp.idx;
+                ok = ok && wait(bar(FULL + rp.idx), rp.phase);
+                fence_after();
+                rp.next(kPreRing);
+            };
+            // scores = q tile x K; K-major both: 16 values are 32 bytes into a 128-byte row
+            auto qk = [&](uint32_t d, uint32_t q, uint32_t slot, bool acc) {
+                const uint64_t da = smem_desc_sw128(q, 16u, 1024u), db = smem_desc_sw128(ring + slot * TILE, 16u, 1024u);
+#pragma unroll
+                for (int k = 0; k < D / 16; k++) {
+                    const uint64_t off = (uint64_t)(((k >> 2) * HALF + (k & 3) * 32u) >> 4);
+                    umma_f16(d, da + off, db + off, IQK, (k > 0 || acc) ? 1u : 0u);
+                }
+            };
+            // output = e x V; V N-major: 16 keys are 2048 bytes, the next 64 values HALF further
+            auto pv = [&](uint32_t d, uint32_t e, uint32_t slot, bool acc) {
+                const uint64_t db = smem_desc_sw128(ring + slot * TILE, HALF, 1024u);
+#pragma unroll
+                for (int k = 0; k < kPreKeys / 16; k++)
+                    umma_f16_ts(d, e + 8u * k, db + (uint64_t)(k * 2048u >> 4), IPV, (k > 0 || acc) ? 1u : 0u);
+            };
+            uint32_t ks, vs;
+            if constexpr (SPLIT) {
+                auto scores = [&](int j) {
+                    take(ks);
+                    if (!ok) return;
+                    const uint32_t d = tmem + kS + 128u * (j & 1);
+                    qk(d, q_tile, ks, false);
+                    qk(d, q_tile + TILE, ks, true);
+                    umma_commit(bar(SF + (j & 1)));
+                    umma_commit(bar(EMPTY + ks));
+                };
+                scores(0);
+                if (ok && n > 1) scores(1);
+                for (int j = 0; j < n && ok; j++) {
+                    const uint32_t b = j & 1, ph = (j >> 1) & 1;
+                    take(vs);
+                    if (ok && j >= 2) ok = wait(bar(TE + b), ph ^ 1u);
+                    if (ok) ok = wait(bar(PF + b), ph);
+                    if (!ok) break;
+                    fence_after();
+                    const uint32_t d = tmem + kO + 128u * b, e = tmem + kS + 128u * b;
+                    pv(d, e, vs, false);
+                    pv(d, e + 64u, vs, true);
+                    umma_commit(bar(TF + b));
+                    umma_commit(bar(EMPTY + vs));
+                    if (j + 2 < n) scores(j + 2);
+                }
+            } else {
+                take(ks);
+                if (ok) {
+                    qk(tmem + kS, q_tile, ks, false);
+                    umma_commit(bar(SF));
+                    if (two) {
+                        qk(tmem + kS + 128u, q_tile + TILE, ks, false);
+                        umma_commit(bar(SF + 1));
+                    }
+                    umma_commit(bar(EMPTY + ks));
+                }
+                for (int j = 0; j < n && ok; j++) {
+                    const uint32_t ph = j & 1;
+                    const bool more = j + 1 < n;
+                    take(vs);
+                    if (ok) ok = wait(bar(PF), ph);
+                    if (!ok) break;
+                    fence_after();
+                    pv(tmem + kO, tmem + kS, vs, j > 0);
+                    if (!two) umma_commit(bar(EMPTY + vs));
+                    if (more) {
+                        take(ks);
+                        if (!ok) break;
+                        qk(tmem + kS, q_tile, ks, false);
+                        umma_commit(bar(SF));
+                        if (!two) umma_commit(bar(EMPTY + ks));
+                    } else {
+                        umma_commit(bar(TF));
+                    }
+                    if (two) {
+                        ok = wait(bar(PF + 1), ph);
+                        if (!ok) break;
+                        fence_after();
+                        pv(tmem + kO + 128u, tmem + kS + 128u, vs, j > 0);
+                        umma_commit(bar(EMPTY + vs));
+                        if (more) {
+                            qk(tmem + kS + 128u, q_tile + TILE, ks, false);
+                            umma_commit(bar(SF + 1));
+                            umma_commit(bar(EMPTY + ks));
+                        } else {
+                            umma_commit(bar(TF + 1));
+                        }
+                    }
+                }
+            }
+            // every product issued has finished before TMEM is given back
+            umma_commit(bar(DR));
+            if (!mbar_wait_bounded(bar(DR), 0, kPreWaitNs)) atomicExch(&g_kv8_prefill_status, kStatusTimeout);
+        }
+        __syncwarp();
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegScore));
+        const uint32_t my = tmem + ((uint32_t)(32 * (warp & 3)) << 16);  // the warp's lanes
+        // the rows' outputs: `part` and `stat` of this range, or out
+        float *part = p.part + (tile * p.splits + split) * ROWS * D;
+        float *stat = p.stat + (tile * p.splits + split) * ROWS * 2;
+        const int row = SPLIT ? t : 128 * wg + t;
+        T *out_row = nullptr;
+        if (r0 + row < rows_all)
+            out_row = static_cast<T *>(p.out) + (int64_t)(s.first + (r0 + row) / p.g) * p.ot +
+                      (int64_t)(kvh * p.g + (r0 + row) % p.g) * D;
+        auto put = [&](int c, float (&v)[8], float l) {  // eight values from dimension c
+            if (!out_row) return;
+            if (active > 1) {
+                float4 *d = reinterpret_cast<float4 *>(part + (int64_t)row * D + c);
+                d[0] = make_float4(v[0], v[1], v[2], v[3]);
+                d[1] = make_float4(v[4], v[5], v[6], v[7]);
+            } else {
+                const float inv = l == 0.f ? 0.f : kOut / l;
+#pragma unroll
+                for (int u = 0; u < 8; u++) v[u] *= inv;
+                store_act<T, 8>(out_row + c, v, p.vec);
+            }
+        };
+        const float nan = __int_as_float(0x7fc00000);
+        if (wg == 0 || (!SPLIT && two)) {
+            // ---- scores to e ----
+            float m = -INFINITY, l = 0.f;
+            const int warp_hi = __reduce_min_sync(0xffffffffu, see_hi), warp_lo = __reduce_max_sync(0xffffffffu, see_lo);
+            bool ok = true;
+            for (int j = 0; j < n && ok; j++) {
+                const uint32_t b = SPLIT ? (j & 1) : wg;
+                const uint32_t ph = SPLIT ? (j >> 1) & 1 : j & 1;
+                ok = wait_warp(bar(SF + b), ph);
+                if (!ok) break;
+                fence_after();
+                const uint32_t sc = my + kS + 128u * b;
+                uint32_t x[4][32];
+#pragma unroll
+                for (int i = 0; i < 4; i++) tmem_ld32(x[i], sc + 32u * i);
+                float kf[kPreBlocks], lv[kPreBlocks];
+#pragma unroll
+                for (int i = 0; i < kPreBlocks; i++) {
+                    kf[i] = fmaxf(scales[j & 3][0][i] * rf, 1.4e-45f);  // above 0: -inf stays -inf
+                    lv[i] = scales[j & 3][1][i];
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) tmem_wait_ld(x[i]);
+                const int key = k_lo + j * kPreKeys;
+                if (key < warp_lo || key + kPreKeys > warp_hi) {
+#pragma unroll
+                    for (int i = 0; i < kPreKeys; i++)
+                        if (key + i < see_lo || key + i >= see_hi) x[i / 32][i % 32] = 0xff800000u;  // -inf
+                }
+                // the tile's maximum of x + lv
+                float mx = m;
+#pragma unroll
+                for (int i = 0; i < kPreBlocks; i++) {
+                    float a = __uint_as_float(x[i / 2][16 * (i % 2)]);
+#pragma unroll
+                    for (int u = 1; u < kKv8Block; u++) a = fmaxf(a, __uint_as_float(x[i / 2][16 * (i % 2) + u]));
+                    mx = fmaxf(mx, fmaf(a, kf[i], lv[i]));
+                }
+                float al = 1.f;
+                if constexpr (SPLIT) {
+                    al = mx == -INFINITY ? 1.f : ex2p(m - mx);
+                    alpha[j & 3][t] = al;
+                    m = mx;
+                } else {
+                    // raised only when e would pass 2^8: the output stays as it is otherwise
+                    const bool raise = mx > m + 8.f;
+                    if (__any_sync(0xffffffffu, raise)) {
+                        if (raise) {
+                            al = ex2p(m - mx);
+                            m = mx;
+                        }
+                        if (j > 0) {
+#pragma unroll
+                            for (int i = 0; i < D / 8; i++) {
+                                uint32_t o[8];
+                                tmem_ld8(o, my + kO + 128u * wg + 8u * i);
+                                tmem_wait_ld(o);
+#pragma unroll
+                                for (int u = 0; u < 8; u++) o[u] = __float_as_uint(__uint_as_float(o[u]) * al);
+                                tmem_st8(my + kO + 128u * wg + 8u * i, o);
+                            }
+                        }
+                    }
+                }
+                l *= al;
+                const float off = m == -INFINITY ? 0.f : m - kUp;
+#pragma unroll
+                for (int i = 0; i < kPreBlocks; i++) {
+                    const float d = lv[i] - off;
+                    float sum = 0.f;
+#pragma unroll
+                    for (int u = 0; u < kKv8Block; u++) {
+                        uint32_t &y = x[i / 2][16 * (i % 2) + u];
+                        const float e = ex2p(fmaf(__uint_as_float(y), kf[i], d));
+                        sum += e;
+                        y = __float_as_uint(e);
+                    }
+                    l = fmaf(sum, scales[j & 3][2][i], l);
+                }
+                // e as float16 over the scores: 64 columns (SPLIT: the low parts in 64 more)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    uint32_t hp[16];
+#pragma unroll
+                    for (int u = 0; u < 16; u++)
+                        hp[u] = pack_half(__uint_as_float(x[i][2 * u]), __uint_as_float(x[i][2 * u + 1]));
+                    tmem_st16(sc + 16u * i, hp);
+                    if constexpr (SPLIT) {
+                        uint32_t lp[16];
+#pragma unroll
+                        for (int u = 0; u < 16; u++) {
+                            const float2 back = unpack_half(hp[u]);
+                            lp[u] = pack_half(__uint_as_float(x[i][2 * u]) - back.x, __uint_as_float(x[i][2 * u + 1]) - back.y);
+                        }
+                        tmem_st16(sc + 64u + 16u * i, lp);
+                    }
+                }
+                tmem_wait_st();
+                fence_before();
+                arrive(bar(PF + b));
+            }
+            if constexpr (SPLIT) {
+                lsum[t] = l, msum[t] = m;
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+            } else {
+                const bool got = n > 0 && wait_warp(bar(TF + wg), 0);
+                fence_after();
+                if (bad_flag || abort_flag) l = nan;
+                if (active > 1 && out_row) stat[2 * row] = m, stat[2 * row + 1] = l;
+#pragma unroll
+                for (int i = 0; i < D / 32; i++) {
+                    uint32_t o[32];
+                    if (got) {
+                        tmem_ld32(o, my + kO + 128u * wg + 32u * i);
+                        tmem_wait_ld(o);
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < 32; u++) o[u] = 0;
+                    }
+#pragma unroll
+                    for (int c = 0; c < 32; c += 8) {
+                        float v[8];
+#pragma unroll
+                        for (int u = 0; u < 8; u++) v[u] = __uint_as_float(o[c + u]);
+                        put(32 * i + c, v, l);
+                    }
+                }
+            }
+        } else if constexpr (SPLIT) {
+            // ---- the key tiles' outputs, added in float32 ----
+            float acc[D];
+#pragma unroll
+            for (int i = 0; i < D; i++) acc[i] = 0.f;
+            for (int j = 0; j < n; j++) {
+                const uint32_t b = j & 1;
+                if (!wait_warp(bar(TF + b), (j >> 1) & 1)) break;
+                fence_after();
+                const float al = alpha[j & 3][t];
+#pragma unroll
+                for (int i = 0; i < D / 32; i++) {
+                    uint32_t o[32];
+                    tmem_ld32(o, my + kO + 128u * b + 32u * i);
+                    tmem_wait_ld(o);
+#pragma unroll
+                    for (int u = 0; u < 32; u++) acc[32 * i + u] = fmaf(acc[32 * i + u], al, __uint_as_float(o[u]));
+                }
+                fence_before();
+                arrive(bar(TE + b));
+            }
+            // l and M are warpgroup 0's: its last e came before the last output
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            float l = lsum[t];
+            if (bad_flag || abort_flag) l = nan;
+            if (active > 1 && out_row) stat[2 * row] = msum[t], stat[2 * row + 1] = l;
+#pragma unroll
+            for (int c = 0; c < D; c += 8) {
+                float v[8];
+#pragma unroll
+                for (int u = 0; u < 8; u++) v[u] = acc[c + u];
+                put(c, v, l);
+            }
+        }
+    }
+    fence_before();
+    if (active > 1) __threadfence();
+    __syncthreads();
+    if (warp == 12) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    }
+    if (tid == 0) {
+        if (bad_flag) atomicExch(&g_kv8_prefill_status, VKQ_ERR_INVALID_ARGUMENT);
+        last = active > 1 && atomicAdd(p.count + tile, 1u) == (unsigned)active - 1u;
+    }
+    __syncthreads();
+    if (!last) return;
+    // the ranges' parts, in order
+    __threadfence();
+    if (tid == 0) p.count[tile] = 0;
+    const float *part = p.part + tile * p.splits * ROWS * D, *stat = p.stat + tile * p.splits * ROWS * 2;
+    const float nan = __int_as_float(0x7fc00000);
+    for (int i = tid; i < ROWS * D / 4; i += kPreThreads) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4;
+        if (r0 + r >= rows_all) break;
+        float mx = -INFINITY;
+        for (int w = 0; w < active; w++) mx = fmaxf(mx, __ldcg(stat + (w * ROWS + r) * 2));
+        float sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int w = 0; w < active; w++) {
+            const float2 ms = __ldcg(reinterpret_cast<const float2 *>(stat + (w * ROWS + r) * 2));
+            const float4 v = __ldcg(reinterpret_cast<const float4 *>(part + ((int64_t)w * ROWS + r) * D + d));
+            const float k = ms.x == -INFINITY ? (ms.y == ms.y ? 0.f : nan) : ex2p(ms.x - mx);
+            sum += k * ms.y;
+            acc[0] += k * v.x, acc[1] += k * v.y, acc[2] += k * v.z, acc[3] += k * v.w;
+        }
+        const float inv = sum == 0.f ? 0.f : kOut / sum;
+#pragma unroll
+        for (int z = 0; z < 4; z++) acc[z] *= inv;
+        store_act<T, 4>(static_cast<T *>(p.out) + (int64_t)(s.first + (r0 + r) / p.g) * p.ot +
+                            (int64_t)(kvh * p.g + (r0 + r) % p.g) * D + d,
+                        acc, p.vec);
+    }
+}
+
+template <typename T, int D>
+static const void *prefill_fn(bool e4m3) {
+    return e4m3 ? (const void *)kv8_prefill_kernel<T, D, true> : (const void *)kv8_prefill_kernel<T, D, false>;
+}
+template <typename T>
+static const void *prefill_fn(int D, bool e4m3) {
+    return D == 64 ? prefill_fn<T, 64>(e4m3) : prefill_fn<T, 128>(e4m3);
+}
+
+Kv8Plan kv8_prefill_plan(const vkq_kv8_cache &c, const vkq_kv8_batch &b, int dtype, int64_t heads, int causal,
+                         int64_t window, int sms) {
+    Kv8Plan q{};
+    q.rows = dtype == VKQ_F32 ? 128 : 256;
+    const int64_t g = heads / c.kv_heads;
+    q.row_tiles = (int)((b.max_tokens * g + q.rows - 1) / q.rows);
+    q.tiles = b.batch * c.kv_heads * q.row_tiles;
+    int64_t keys = b.max_len;
+    if (causal && window > 0) {
+        const int64_t w = window + (q.rows + g - 1) / g + kKv8Block;
+        if (w < keys) keys = w;
+    }
+    if (keys < 1) keys = 1;
+    // one CTA an SM: ranges of at least four key tiles until there are two waves
+    int64_t splits = 2 * (int64_t)sms / q.tiles;
+    const int64_t most = (keys + 4 * kPreKeys - 1) / (4 * kPreKeys);
+    if (splits > most) splits = most;
+    if (splits > 64) splits = 64;
+    if (splits < 1 || q.tiles > kHeadCounters) splits = 1;
+    int64_t chunk = (keys + splits - 1) / splits;
+    chunk = (chunk + kPreKeys - 1) / kPreKeys * kPreKeys;
+    q.chunk = (int)chunk;
+    q.splits = (int)((keys + chunk - 1) / chunk);
+    if (q.splits > 1) {
+        q.part_floats = (size_t)(q.tiles * q.splits * q.rows * c.head_dim);
+        q.stat_floats = (size_t)(q.tiles * q.splits * q.rows * 2);
+    }
+    return q;
+}
+
+cudaError_t kv8_prefill(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_batch &b, const Kv8AttentionArgs &a,
+                        const Kv8Plan &q, cudaStream_t s) {
+    PrefillParams p{};
+    p.pool = kv8_pool(c, layer);
+    p.batch = kv8_batch(b);
+    p.q = a.q, p.out = a.out, p.qt = a.q_token, p.ot = a.out_token;
+    p.heads = (int)a.heads, p.g = (int)(a.heads / c.kv_heads);
+    p.row_tiles = q.row_tiles, p.splits = q.splits, p.chunk = q.chunk;
+    p.f = a.scale * 1.4426950408889634f;
+    p.causal = a.causal, p.window = a.causal ? (int)a.window : 0;
+    const int size = act_bytes(a.dtype);
+    p.vec = (((uintptr_t)a.q | (uintptr_t)a.out | (uintptr_t)(a.q_token * size) | (uintptr_t)(a.out_token * size)) & 15u) == 0;
+    p.count = static_cast<unsigned *>(a.workspace);
+    p.part = reinterpret_cast<float *>(static_cast<char *>(a.workspace) + kWorkspaceCounterHead);
+    p.stat = p.part + q.part_floats;
+    const void *fn = a.dtype == VKQ_F32   ? prefill_fn<float>(c.head_dim, p.pool.e4m3)
+                     : a.dtype == VKQ_F16 ? prefill_fn<__half>(c.head_dim, p.pool.e4m3)
+                                          : prefill_fn<__nv_bfloat16>(c.head_dim, p.pool.e4m3);
+    const size_t smem = (size_t)(2 + kPreRing) * 128 * c.head_dim * 2 + 1024;
+    cudaError_t e = kernel_smem(fn, smem, true);
+    if (e != cudaSuccess) return e;
+    // the warpgroups' register split draws on what the block is launched with
+    static std::atomic<const void *> checked[12];
+    std::atomic<const void *> &seen = checked[(a.dtype == VKQ_F32 ? 0 : a.dtype == VKQ_F16 ? 1 : 2) * 4 +
+                                              (c.head_dim == 128 ? 2 : 0) + (p.pool.e4m3 ? 1 : 0)];
+    if (seen.load() != fn) {
+        cudaFuncAttributes fa;
+        e = cudaFuncGetAttributes(&fa, fn);
+        if (e != cudaSuccess) return e;
+        if (fa.numRegs * 4 < 2 * kRegScore + kRegConvert + kRegIssue) return cudaErrorLaunchOutOfResources;
+        seen.store(fn);
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(q.tiles * q.splits));
+    cfg.blockDim = dim3(kPreThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    void *args[] = {(void *)&p};
+    return cudaLaunchKernelExC(&cfg, fn, args);
+}
+
+int kv8_prefill_read_status() {
+    int v = 0, zero = 0;
+    if (cudaMemcpyFromSymbol(&v, g_kv8_prefill_status, sizeof(int)) != cudaSuccess) return -1;
+    cudaMemcpyToSymbol(g_kv8_prefill_status, &zero, sizeof(int));
+    return v;
+}
+
+}  // namespace vkq

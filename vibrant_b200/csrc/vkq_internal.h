@@ -211,6 +211,20 @@ struct Kv8AttentionArgs {
     int64_t window;
     void *workspace;
 };
+// How an attention call is cut: tiles of rows, ranges of keys, and the floats
+// that the ranges' parts take in the workspace past the counters.
+struct Kv8Plan {
+    int rows, row_tiles, splits, chunk;
+    int64_t tiles;
+    size_t part_floats, stat_floats;
+};
+constexpr uint32_t kHeadCounters = (uint32_t)(kWorkspaceCounterHead / sizeof(unsigned));
+// Many query rows (kv8_prefill.cu), chosen by kv8_attention.
+Kv8Plan kv8_prefill_plan(const vkq_kv8_cache &c, const vkq_kv8_batch &b, int dtype, int64_t heads, int causal,
+                         int64_t window, int sms);
+cudaError_t kv8_prefill(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_batch &b, const Kv8AttentionArgs &a,
+                        const Kv8Plan &q, cudaStream_t s);
+int kv8_prefill_read_status();
 size_t kv8_attention_workspace(const vkq_kv8_cache &c, const vkq_kv8_batch &b, int dtype, int64_t heads, int causal,
                                int64_t window, int device);
 cudaError_t kv8_attention(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_batch &b, const Kv8AttentionArgs &a,
