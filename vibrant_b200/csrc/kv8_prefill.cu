@@ -53,7 +53,12 @@ constexpr int kPreBlocks = kPreKeys / kKv8Block;  // and its scale blocks
 constexpr int kPreRing = 4;
 constexpr uint64_t kPreWaitNs = 2000000000ull;
 // registers a thread of warpgroups 0 and 1, of 2, of 3: at most 4 x 128 in all
-constexpr int kRegScore = 184, kRegConvert = 104, kRegIssue = 40;
+// (float32: warpgroup 1 holds a row's output)
+template <bool SPLIT> struct PreRegs {
+    static constexpr int score = SPLIT ? 176 : 160, convert = SPLIT ? 112 : 120, issue = SPLIT ? 48 : 64;
+    static_assert(2 * score + convert + issue <= 512, "more than the launch has");
+    static_assert(score > 128 && convert < 128 && issue < 128, "setmaxnreg.inc grows, setmaxnreg.dec shrinks");
+};
 
 struct PrefillParams {
     Kv8Pool pool;
@@ -313,13 +318,16 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
     const uint32_t tmem = tmem_slot;
 
     auto wait = [&](uint32_t b, uint32_t parity) -> bool {
-        if (mbar_wait_spin(b, parity, kPreWaitNs)) return true;
+        if (mbar_wait_poll(b, parity, kPreWaitNs)) return true;
         atomicExch(&g_kv8_prefill_status, kStatusTimeout);
         abort_flag = 1;
         return false;
     };
-    // for whole warps: no lane goes on alone
-    auto wait_warp = [&](uint32_t b, uint32_t parity) -> bool { return __all_sync(0xffffffffu, wait(b, parity)); };
+    // for whole warps: one lane polls
+    auto wait_warp = [&](uint32_t b, uint32_t parity) -> bool {
+        const int ok = lane == 0 ? wait(b, parity) : 0;
+        return __shfl_sync(0xffffffffu, ok, 0) != 0;
+    };
     auto arrive = [&](uint32_t b) {  // once for the warp, after all its lanes
         __syncwarp();
         if (lane == 0) mbar_arrive(b);
@@ -331,94 +339,93 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
     // asked for before the output of the one before).
     if (wg == 2) {
         // ---- codes to float16 tiles ----
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegConvert));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PreRegs<SPLIT>::convert));
         constexpr int PER = kPreKeys * D / 16 / 128;  // 16-byte pieces of a tile that a thread takes: 8 or 4
         constexpr int CPR = D / 16;                   // pieces of a row
         constexpr int RSTEP = 128 / CPR;              // rows between a thread's pieces: 16 or 32
         const int row0 = t / CPR, ch = t % CPR;
         const int per_page = p.pool.page / kKv8Block;
-        auto load = [&](int j, bool is_v, uint4 (&raw)[PER]) {
-            const uint8_t *codes = is_v ? p.pool.v : p.pool.k;
+        const int64_t head_off = (int64_t)kvh * p.pool.page;
+        // Three tiles are under way, so that neither the table's nor the pages'
+        // latency is waited for: the page numbers of the one after next (lane b
+        // looks up block b: as `block` codes into the pool, -1 for none), the
+        // codes of the next, the conversion of this one.
+        struct Item {
+            int j, k_done, v_done;  // key tile; K and V tiles up to and with this one
+            bool is_v;
+        };
+        auto after = [&](const Item &a) {
+            Item b;
+            b.is_v = SPLIT ? !(a.k_done < n && a.k_done < a.v_done + 2) : a.v_done < a.k_done;
+            b.j = b.is_v ? a.v_done : a.k_done;
+            b.k_done = a.k_done + !b.is_v, b.v_done = a.v_done + b.is_v;
+            return b;
+        };
+        // row of the pool ([page][kv head][token]) where the lane's block starts, -1 for none
+        auto look = [&](const Item &a) -> int64_t {
+            const int key = k_lo + a.j * kPreKeys + (lane & (kPreBlocks - 1)) * kKv8Block;
+            if (a.j >= n || key >= k_hi) return -1;
+            const int blk = key / kKv8Block, lp = blk / per_page;
+            const int id = kv8_page(p.pool, s, lp);
+            if (id < 0) bad_flag = 1;
+            return id < 0 ? -1 : (int64_t)id * p.pool.kv_heads * p.pool.page + head_off + (blk - lp * per_page) * kKv8Block;
+        };
+        auto load = [&](const Item &a, int64_t at, uint4 (&raw)[PER], float &ks, float &vs) {
+            const uint8_t *codes = (a.is_v ? p.pool.v : p.pool.k) + (row0 % kKv8Block) * D + ch * 16;
+            const int key = k_lo + a.j * kPreKeys + row0;
 #pragma unroll
             for (int k = 0; k < PER; k++) {
-                const int row = row0 + k * RSTEP, key = k_lo + j * kPreKeys + row;
+                const int64_t r = __shfl_sync(0xffffffffu, at, (row0 + k * RSTEP) / kKv8Block);
+                const bool ok = r >= 0 && key + k * RSTEP < k_hi;
                 raw[k] = make_uint4(0, 0, 0, 0);
-                if (key < k_hi) {
-                    const int blk = key / kKv8Block, lp = blk / per_page;
-                    const int id = kv8_page(p.pool, s, lp);
-                    if (id < 0) {
-                        bad_flag = 1;
-                    } else {
-                        const int64_t r = ((int64_t)id * p.pool.kv_heads + kvh) * p.pool.page + (key - lp * p.pool.page);
-                        raw[k] = *reinterpret_cast<const uint4 *>(codes + r * D + ch * 16);
-                    }
-                }
+                if (ok) raw[k] = __ldg(reinterpret_cast<const uint4 *>(codes + r * D));
             }
-        };
-        auto load_scales = [&](int j, float &ks, float &vs) {  // threads 0 .. 7
+            // lane b of the first warp: the scales of block b
             ks = vs = 1.f;
-            const int key = k_lo + j * kPreKeys + t * kKv8Block;
-            if (t < kPreBlocks && key < k_hi) {
-                const int blk = key / kKv8Block, lp = blk / per_page;
-                const int id = kv8_page(p.pool, s, lp);
-                if (id >= 0) {
-                    const int64_t e = ((int64_t)id * p.pool.kv_heads + kvh) * per_page + (blk - lp * per_page);
-                    ks = p.pool.ks[e];
-                    vs = p.pool.vs[e];
-                }
-            }
+            if (warp == 8 && !a.is_v && at >= 0) ks = p.pool.ks[at / kKv8Block], vs = p.pool.vs[at / kKv8Block];
         };
-        uint4 raw[PER], next[PER];
-        float ks, vs, ks_n = 1.f, vs_n = 1.f;
-        int j = 0;
-        bool is_v = false;
-        if (n > 0) {
-            load(0, false, raw);
-            load_scales(0, ks, vs);
-        }
-        int k_done = 0, v_done = 0;  // tiles handed over
+        uint4 raw[2][PER];
+        float ks[2], vs[2];
+        Item item{0, 1, 0, false}, next = after(item);
+        load(item, look(item), raw[0], ks[0], vs[0]);
+        int64_t at = look(next);
         RingPos rp;
-        for (int it = 0; it < 2 * n; it++) {
-            // the tile after this one
-            int kd = k_done + !is_v, vd = v_done + is_v;
-            bool nv;
-            if (SPLIT) nv = !(kd < n && kd < vd + 2);
-            else nv = vd < kd;
-            const int nj = nv ? vd : kd;
-            if (it + 1 < 2 * n) {
-                load(nj, nv, next);
-                if (!nv) load_scales(nj, ks_n, vs_n);
-            }
-            if (rp.uses >= (uint32_t)kPreRing && !wait_warp(bar(EMPTY + rp.idx), rp.phase ^ 1u)) break;
-            const uint32_t dst = ring + rp.idx * TILE;
+        bool ok = true;
+        for (int it = 0; it < 2 * n && ok; it += 2) {
 #pragma unroll
-            for (int k = 0; k < PER; k++) {
-                uint32_t h[8];
-                codes_to_half<E4M3>(raw[k], h);
-                const int row = row0 + k * RSTEP;
-                const uint32_t a = dst + tile_off(row, 2 * ch), b = dst + tile_off(row, 2 * ch + 1);
-                // eight lanes of one row: pieces of both halves fall into different banks
-                const bool odd = ch >= 4;
-                sts128(odd ? b : a, odd ? h[4] : h[0], odd ? h[5] : h[1], odd ? h[6] : h[2], odd ? h[7] : h[3]);
-                sts128(odd ? a : b, odd ? h[0] : h[4], odd ? h[1] : h[5], odd ? h[2] : h[6], odd ? h[3] : h[7]);
-            }
-            if (!is_v && t < kPreBlocks) {
-                scales[j & 3][0][t] = ks;
-                scales[j & 3][1][t] = __log2f(vs);
-                scales[j & 3][2][t] = 1.f / vs;
-            }
-            fence_async();
-            arrive(bar(FULL + rp.idx));
-            rp.next(kPreRing);
-            k_done = kd, v_done = vd;
-            j = nj, is_v = nv;
+            for (int x = 0; x < 2; x++) {  // 2 n tiles: an even number
+                load(next, at, raw[x ^ 1], ks[x ^ 1], vs[x ^ 1]);
+                const Item later = after(next);
+                at = look(later);
+                ok = ok && (rp.uses < (uint32_t)kPreRing || wait_warp(bar(EMPTY + rp.idx), rp.phase ^ 1u));
+                if (!ok) break;
+                const uint32_t dst = ring + rp.idx * TILE;
 #pragma unroll
-            for (int k = 0; k < PER; k++) raw[k] = next[k];
-            if (!nv) ks = ks_n, vs = vs_n;
+                for (int k = 0; k < PER; k++) {
+                    uint32_t h[8];
+                    codes_to_half<E4M3>(raw[x][k], h);
+                    const int row = row0 + k * RSTEP;
+                    const uint32_t a = dst + tile_off(row, 2 * ch), b = dst + tile_off(row, 2 * ch + 1);
+                    // eight lanes of one row: pieces of both halves fall into different banks
+                    const bool odd = ch >= 4;
+                    sts128(odd ? b : a, odd ? h[4] : h[0], odd ? h[5] : h[1], odd ? h[6] : h[2], odd ? h[7] : h[3]);
+                    sts128(odd ? a : b, odd ? h[0] : h[4], odd ? h[1] : h[5], odd ? h[2] : h[6], odd ? h[3] : h[7]);
+                }
+                if (warp == 8 && lane < kPreBlocks && !item.is_v) {
+                    scales[item.j & 3][0][lane] = ks[x];
+                    scales[item.j & 3][1][lane] = __log2f(vs[x]);
+                    scales[item.j & 3][2][lane] = 1.f / vs[x];
+                }
+                fence_async();
+                arrive(bar(FULL + rp.idx));
+                rp.next(kPreRing);
+                item = next;
+                next = later;
+            }
         }
     } else if (wg == 3) {
         // ---- the products ----
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegIssue));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PreRegs<SPLIT>::issue));
         if (warp == 12 && lane == 0 && n > 0) {
             constexpr uint32_t IQK = idesc_f16(kPreKeys, false), IPV = idesc_f16(D, true);
             RingPos rp;
@@ -432,18 +439,18 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
             // scores = q tile x K; K-major both: 16 values are 32 bytes into a 128-byte row
             auto qk = [&](uint32_t d, uint32_t q, uint32_t slot, bool acc) {
                 const uint64_t da = smem_desc_sw128(q, 16u, 1024u), db = smem_desc_sw128(ring + slot * TILE, 16u, 1024u);
-#pragma unroll
+#pragma unroll 1
                 for (int k = 0; k < D / 16; k++) {
                     const uint64_t off = (uint64_t)(((k >> 2) * HALF + (k & 3) * 32u) >> 4);
                     umma_f16(d, da + off, db + off, IQK, (k > 0 || acc) ? 1u : 0u);
                 }
             };
-            // output = e x V; V N-major: 16 keys are 2048 bytes, the next 64 values HALF further
+            // output = e x V; e: 16 keys are 8 of every 32 columns' first 16; V N-major: 16 keys are 2048 bytes, the next 64 values HALF further
             auto pv = [&](uint32_t d, uint32_t e, uint32_t slot, bool acc) {
                 const uint64_t db = smem_desc_sw128(ring + slot * TILE, HALF, 1024u);
-#pragma unroll
+#pragma unroll 1
                 for (int k = 0; k < kPreKeys / 16; k++)
-                    umma_f16_ts(d, e + 8u * k, db + (uint64_t)(k * 2048u >> 4), IPV, (k > 0 || acc) ? 1u : 0u);
+                    umma_f16_ts(d, e + 32u * (k >> 1) + 8u * (k & 1), db + (uint64_t)(k * 2048u >> 4), IPV, (k > 0 || acc) ? 1u : 0u);
             };
             uint32_t ks, vs;
             if constexpr (SPLIT) {
@@ -467,7 +474,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
                     fence_after();
                     const uint32_t d = tmem + kO + 128u * b, e = tmem + kS + 128u * b;
                     pv(d, e, vs, false);
-                    pv(d, e + 64u, vs, true);
+                    pv(d, e + 16u, vs, true);
                     umma_commit(bar(TF + b));
                     umma_commit(bar(EMPTY + vs));
                     if (j + 2 < n) scores(j + 2);
@@ -523,7 +530,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
         }
         __syncwarp();
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegScore));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PreRegs<SPLIT>::score));
         const uint32_t my = tmem + ((uint32_t)(32 * (warp & 3)) << 16);  // the warp's lanes
         // the rows' outputs: `part` and `stat` of this range, or out
         float *part = p.part + (tile * p.splits + split) * ROWS * D;
@@ -559,31 +566,35 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
                 if (!ok) break;
                 fence_after();
                 const uint32_t sc = my + kS + 128u * b;
-                uint32_t x[4][32];
-#pragma unroll
-                for (int i = 0; i < 4; i++) tmem_ld32(x[i], sc + 32u * i);
-                float kf[kPreBlocks], lv[kPreBlocks];
-#pragma unroll
-                for (int i = 0; i < kPreBlocks; i++) {
-                    kf[i] = fmaxf(scales[j & 3][0][i] * rf, 1.4e-45f);  // above 0: -inf stays -inf
-                    lv[i] = scales[j & 3][1][i];
-                }
-#pragma unroll
-                for (int i = 0; i < 4; i++) tmem_wait_ld(x[i]);
                 const int key = k_lo + j * kPreKeys;
-                if (key < warp_lo || key + kPreKeys > warp_hi) {
+                const bool edge = key < warp_lo || key + kPreKeys > warp_hi;
+                const float *kss = scales[j & 3][0], *lvs = scales[j & 3][1], *inv = scales[j & 3][2];
+                // 32 scores (two blocks) at a time, twice: rolled loops, because the
+                // roles' code has to stay in the instruction cache together
+                uint32_t x[32];
+                auto scores = [&](int i) {
+                    tmem_ld32(x, sc + 32u * i);
+                    tmem_wait_ld(x);
+                    if (edge) {
+                        const int k0 = see_lo - key - 32 * i, k1 = see_hi - key - 32 * i;  // visible: [k0, k1)
 #pragma unroll
-                    for (int i = 0; i < kPreKeys; i++)
-                        if (key + i < see_lo || key + i >= see_hi) x[i / 32][i % 32] = 0xff800000u;  // -inf
-                }
+                        for (int u = 0; u < 32; u++)
+                            if (u < k0 || u >= k1) x[u] = 0xff800000u;  // -inf
+                    }
+                };
                 // the tile's maximum of x + lv
                 float mx = m;
+#pragma unroll 1
+                for (int i = 0; i < 4; i++) {
+                    scores(i);
 #pragma unroll
-                for (int i = 0; i < kPreBlocks; i++) {
-                    float a = __uint_as_float(x[i / 2][16 * (i % 2)]);
+                    for (int h = 0; h < 2; h++) {
+                        float a = __uint_as_float(x[16 * h]);
 #pragma unroll
-                    for (int u = 1; u < kKv8Block; u++) a = fmaxf(a, __uint_as_float(x[i / 2][16 * (i % 2) + u]));
-                    mx = fmaxf(mx, fmaf(a, kf[i], lv[i]));
+                        for (int u = 1; u < kKv8Block; u++) a = fmaxf(a, __uint_as_float(x[16 * h + u]));
+                        // the factor above 0: -inf stays -inf
+                        mx = fmaxf(mx, fmaf(a, fmaxf(kss[2 * i + h] * rf, 1.4e-45f), lvs[2 * i + h]));
+                    }
                 }
                 float al = 1.f;
                 if constexpr (SPLIT) {
@@ -599,7 +610,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
                             m = mx;
                         }
                         if (j > 0) {
-#pragma unroll
+#pragma unroll 1
                             for (int i = 0; i < D / 8; i++) {
                                 uint32_t o[8];
                                 tmem_ld8(o, my + kO + 128u * wg + 8u * i);
@@ -613,35 +624,34 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
                 }
                 l *= al;
                 const float off = m == -INFINITY ? 0.f : m - kUp;
-#pragma unroll
-                for (int i = 0; i < kPreBlocks; i++) {
-                    const float d = lv[i] - off;
-                    float sum = 0.f;
-#pragma unroll
-                    for (int u = 0; u < kKv8Block; u++) {
-                        uint32_t &y = x[i / 2][16 * (i % 2) + u];
-                        const float e = ex2p(fmaf(__uint_as_float(y), kf[i], d));
-                        sum += e;
-                        y = __float_as_uint(e);
-                    }
-                    l = fmaf(sum, scales[j & 3][2][i], l);
-                }
-                // e as float16 over the scores: 64 columns (SPLIT: the low parts in 64 more)
-#pragma unroll
+#pragma unroll 1
                 for (int i = 0; i < 4; i++) {
+                    scores(i);
                     uint32_t hp[16];
 #pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const float kf = fmaxf(kss[2 * i + h] * rf, 1.4e-45f), d = lvs[2 * i + h] - off;
+                        float sum = 0.f;
+#pragma unroll
+                        for (int u = 0; u < kKv8Block; u++) {
+                            const float e = ex2p(fmaf(__uint_as_float(x[16 * h + u]), kf, d));
+                            sum += e;
+                            x[16 * h + u] = __float_as_uint(e);
+                        }
+                        l = fmaf(sum, inv[2 * i + h], l);
+                    }
+                    // e as float16 over its scores: 16 columns (SPLIT: the low parts in the 16 after)
+#pragma unroll
                     for (int u = 0; u < 16; u++)
-                        hp[u] = pack_half(__uint_as_float(x[i][2 * u]), __uint_as_float(x[i][2 * u + 1]));
-                    tmem_st16(sc + 16u * i, hp);
+                        hp[u] = pack_half(__uint_as_float(x[2 * u]), __uint_as_float(x[2 * u + 1]));
+                    tmem_st16(sc + 32u * i, hp);
                     if constexpr (SPLIT) {
-                        uint32_t lp[16];
 #pragma unroll
                         for (int u = 0; u < 16; u++) {
                             const float2 back = unpack_half(hp[u]);
-                            lp[u] = pack_half(__uint_as_float(x[i][2 * u]) - back.x, __uint_as_float(x[i][2 * u + 1]) - back.y);
+                            hp[u] = pack_half(__uint_as_float(x[2 * u]) - back.x, __uint_as_float(x[2 * u + 1]) - back.y);
                         }
-                        tmem_st16(sc + 64u + 16u * i, lp);
+                        tmem_st16(sc + 32u * i + 16u, hp);
                     }
                 }
                 tmem_wait_st();
@@ -818,7 +828,7 @@ cudaError_t kv8_prefill(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_bat
         cudaFuncAttributes fa;
         e = cudaFuncGetAttributes(&fa, fn);
         if (e != cudaSuccess) return e;
-        if (fa.numRegs * 4 < 2 * kRegScore + kRegConvert + kRegIssue) return cudaErrorLaunchOutOfResources;
+        if (fa.numRegs * kPreThreads < 512 * 128) return cudaErrorLaunchOutOfResources;
         seen.store(fn);
     }
     cudaLaunchConfig_t cfg{};
