@@ -5,10 +5,11 @@
 // head, as in kv8_attention.cu, so the heads of a group share every key tile.
 // A CTA (one per SM, four warpgroups) takes one tile of rows and a range of
 // keys in tiles of 128:
-//   warpgroup 2 turns the pages' codes into float16 K and V tiles in shared
-//     memory (exact; 128-byte swizzle, one layout read K-major as K and
-//     MN-major as V), a ring of four;
-//   one warp of warpgroup 3 issues the products;
+//   a warp of warpgroup 3 looks the tiles' pages up and copies their codes to
+//     shared memory, 16 tokens of a head (1 or 2 KB) a bulk copy, a ring of three;
+//   warpgroup 2 turns them into float16 K and V tiles (exact; 128-byte swizzle,
+//     one layout read K-major as K and MN-major as V), a ring of three;
+//   another warp of warpgroup 3 issues the products;
 //   warpgroups 0 and 1 work on the scores, a thread a row.
 // The block scales never touch the operands.  With x = f ks (q . ck) the
 // score of a key in units of log2 and lv = log2 vs,
@@ -50,8 +51,9 @@ static __device__ int g_kv8_prefill_status;
 constexpr int kPreThreads = 512;
 constexpr int kPreKeys = 128;                    // keys of a tile
 constexpr int kPreBlocks = kPreKeys / kKv8Block;  // and its scale blocks
-constexpr int kPreRing = 4;
-constexpr uint64_t kPreWaitNs = 2000000000ull;
+constexpr int kPreRing = 3;  // float16 tiles
+constexpr int kPreRaw = 3;   // tiles of codes
+constexpr uint32_t kPrePolls = 1u << 27;
 // registers a thread of warpgroups 0 and 1, of 2, of 3: at most 4 x 128 in all
 // (float32: warpgroup 1 holds a row's output)
 template <bool SPLIT> struct PreRegs {
@@ -74,17 +76,33 @@ struct PrefillParams {
     unsigned *count;
 };
 
-__device__ __forceinline__ void umma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// Products issued by a whole warp, one lane of which (`one`) is the issuer: the
+// descriptors then stay in uniform registers.  A shared-memory descriptor is
+// given by its low word (address and leading offset) and its constant high one.
+__device__ __forceinline__ void umma_f16(uint32_t d, uint32_t a, uint32_t b, uint32_t hi, uint32_t idesc, uint32_t acc,
+                                         uint32_t one) {
     asm volatile(
-        "{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc));
+        "{ .reg .pred p, q; .reg .b64 x, y; mov.b64 x, {%1, %3}; mov.b64 y, {%2, %3}; setp.ne.b32 p, %5, 0; "
+        "setp.ne.b32 q, %6, 0; @q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %4, p; }" ::"r"(d),
+        "r"(a), "r"(b), "r"(hi), "r"(idesc), "r"(acc), "r"(one));
 }
 // The first operand in TMEM: a row a lane, two float16 a column.
-__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t hi, uint32_t idesc, uint32_t acc,
+                                            uint32_t one) {
     asm volatile(
-        "{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(acc));
+        "{ .reg .pred p, q; .reg .b64 y; mov.b64 y, {%2, %3}; setp.ne.b32 p, %5, 0; setp.ne.b32 q, %6, 0; "
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %4, p; }" ::"r"(d),
+        "r"(a), "r"(b), "r"(hi), "r"(idesc), "r"(acc), "r"(one));
 }
+__device__ __forceinline__ void umma_commit_one(uint32_t bar, uint32_t one) {
+    asm volatile(
+        "{ .reg .pred q; setp.ne.b32 q, %1, 0; "
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0]; }" ::"r"(bar),
+        "r"(one)
+        : "memory");
+}
+__host__ __device__ constexpr uint32_t desc_hi(uint32_t sbo) { return (sbo >> 4) | (1u << 14) | (2u << 29); }
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) { return (addr >> 4) | ((lbo >> 4) << 16); }
 // float16 operands, float32 accumulation, 128 rows; vn: the second operand N-major.
 __host__ __device__ constexpr uint32_t idesc_f16(int n, bool vn) {
     return (1u << 4) | ((vn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
@@ -167,6 +185,15 @@ __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint3
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
+// Polls a phase, kPrePolls times at most (some seconds): a small loop, because
+// the roles' code has to stay in the instruction caches together.
+__device__ __forceinline__ bool poll(uint32_t bar, uint32_t parity) {
+#pragma unroll 1
+    for (uint32_t i = 0; i < kPrePolls; i++)
+        if (mbar_test_wait(bar, parity)) return true;
+    return false;
+}
+
 // 16 codes as 16 float16 (the conversions of kv8_attention.cu).
 template <bool E4M3>
 __device__ __forceinline__ void codes_to_half(const uint4 &raw, uint32_t (&h)[8]) {
@@ -205,10 +232,10 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
     constexpr float kOut = E4M3 ? 256.f : 1.f;      // e4m3 operands are 2^8 too small
     // TMEM columns: the scores (and, over them, e) of half or parity 0 and 1, the outputs
     constexpr uint32_t kS = 0, kO = 256;
-    extern __shared__ __align__(1024) uint8_t smem[];  // two q tiles, the ring
-    __shared__ __align__(8) uint64_t bars[2 * kPreRing + 2 + 2 + 2 + 2 + 1];
-    __shared__ __align__(16) float scales[4][3][kPreBlocks];  // of key tile j & 3: ks, lv, 1 / vs
-    __shared__ float alpha[4][128], lsum[128], msum[128];
+    extern __shared__ __align__(1024) uint8_t smem[];  // two q tiles, the rings
+    __shared__ __align__(8) uint64_t bars[2 * kPreRing + 2 * kPreRaw + 2 + 2 + 2 + 2 + 1];
+    __shared__ __align__(16) float scales[8][3][kPreBlocks];  // of key tile j & 7: ks, lv, 1 / vs
+    __shared__ float alpha[4][128], lsum[128], msum[128], row_f[ROWS];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile uint32_t abort_flag;
     __shared__ uint32_t bad_flag;
@@ -247,13 +274,17 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
     const bool two = !SPLIT && rows_all - r0 > 128;  // the second half has rows
 
     const uint32_t base = (smem_u32addr(smem) + 1023u) & ~1023u;
-    const uint32_t q_tile = base, ring = base + 2 * TILE;
+    const uint32_t q_tile = base, ring = base + 2 * TILE, raw = ring + kPreRing * TILE;
     auto bar = [&](int i) { return smem_u32addr(&bars[i]); };
-    constexpr int FULL = 0, EMPTY = kPreRing, SF = 2 * kPreRing, PF = SF + 2, TF = PF + 2, TE = TF + 2, DR = TE + 2;
+    constexpr int FULL = 0, EMPTY = kPreRing, RF = 2 * kPreRing, RE = RF + kPreRaw, SF = RE + kPreRaw, PF = SF + 2, TF = PF + 2, TE = TF + 2, DR = TE + 2;
     if (tid == 0) {
         for (int i = 0; i < kPreRing; i++) {
             mbar_init(bar(FULL + i), 4);   // a lane of each converting warp
             mbar_init(bar(EMPTY + i), 1);  // commit
+        }
+        for (int i = 0; i < kPreRaw; i++) {
+            mbar_init(bar(RF + i), 1);  // the copies' bytes
+            mbar_init(bar(RE + i), 4);  // a lane of each converting warp
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(bar(SF + i), 1);  // commit: scores
@@ -270,45 +301,38 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32addr(&tmem_slot)));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-    // q: thread t of warpgroup 0 (and 1: the second half) loads its row, scales
-    // it below 2^15 by a power of two and stores its float16 tile (SPLIT: both
-    // parts, warpgroup 0)
-    float rf = 0.f;
-    int see_lo = 0, see_hi = 0;
-    if (wg == 0 || (wg == 1 && !SPLIT)) {
-        const int r = r0 + 128 * wg + t;
+    // q: RT threads load a row, D / RT values each in one burst, scale it below
+    // 2^15 by a power of two and store its float16 tile (SPLIT: both parts)
+    {
+        constexpr int RT = kPreThreads / ROWS, PV = D / RT;
+        const int lr = tid / RT, c0 = (tid % RT) * PV, r = r0 + lr;
         const bool there = r < rows_all;
         const int i = there ? r / p.g : 0, h = kvh * p.g + (there ? r % p.g : 0);
-        const int ps = pos0 + i;
-        see_hi = !there ? 0 : min(p.causal ? ps + 1 : s.len, k_hi);
-        see_lo = p.window > 0 ? ps - p.window + 1 : 0;
-        const T *q = static_cast<const T *>(p.q) + (int64_t)(s.first + i) * p.qt + (int64_t)h * D;
+        float x[PV];
+        load_act<T, PV>(static_cast<const T *>(p.q) + (int64_t)(s.first + i) * p.qt + (int64_t)h * D + c0, x, p.vec);
         float a = 0.f;
-        for (int c = 0; c < D; c += 8) {
-            float x[8];
-            load_act<T, 8>(q + c, x, p.vec);
 #pragma unroll
-            for (int u = 0; u < 8; u++) a = fmaxf(a, fabsf(x[u]));
-        }
+        for (int u = 0; u < PV; u++) a = fmaxf(a, fabsf(x[u]));
+#pragma unroll
+        for (int o = 1; o < RT; o <<= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
         const int e = min(max((int)(__float_as_uint(a) >> 23) - 127, -60), 127);
         const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
-        rf = p.f * __uint_as_float((uint32_t)(e - 14 + 127) << 23) * kOut;
-        const uint32_t dst = q_tile + (SPLIT ? 0u : (uint32_t)wg * TILE);
-        for (int c = 0; c < D; c += 8) {
-            float x[8];
-            load_act<T, 8>(q + c, x, p.vec);
+        if (tid % RT == 0) row_f[lr] = p.f * __uint_as_float((uint32_t)(e - 14 + 127) << 23) * kOut;
+        const uint32_t dst = q_tile + (SPLIT ? 0u : (uint32_t)(lr / 128) * TILE);
+#pragma unroll
+        for (int c = 0; c < PV; c += 8) {
             uint32_t b[4], b2[4];
 #pragma unroll
             for (int u = 0; u < 4; u++) {
-                const float x0 = x[2 * u] * up, x1 = x[2 * u + 1] * up;
+                const float x0 = x[c + 2 * u] * up, x1 = x[c + 2 * u + 1] * up;
                 b[u] = pack_half(x0, x1);
                 if constexpr (SPLIT) {
                     const float2 back = unpack_half(b[u]);
                     b2[u] = pack_half(x0 - back.x, x1 - back.y);
                 }
             }
-            sts128(dst + tile_off(t, c / 8), b[0], b[1], b[2], b[3]);
-            if constexpr (SPLIT) sts128(dst + TILE + tile_off(t, c / 8), b2[0], b2[1], b2[2], b2[3]);
+            sts128(dst + tile_off(lr % 128, (c0 + c) / 8), b[0], b[1], b[2], b[3]);
+            if constexpr (SPLIT) sts128(dst + TILE + tile_off(lr % 128, (c0 + c) / 8), b2[0], b2[1], b2[2], b2[3]);
         }
         fence_async();
     }
@@ -317,15 +341,10 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
     fence_after();
     const uint32_t tmem = tmem_slot;
 
-    auto wait = [&](uint32_t b, uint32_t parity) -> bool {
-        if (mbar_wait_poll(b, parity, kPreWaitNs)) return true;
-        atomicExch(&g_kv8_prefill_status, kStatusTimeout);
-        abort_flag = 1;
-        return false;
-    };
     // for whole warps: one lane polls
     auto wait_warp = [&](uint32_t b, uint32_t parity) -> bool {
-        const int ok = lane == 0 ? wait(b, parity) : 0;
+        int ok = 1;
+        if (lane == 0 && !poll(b, parity)) ok = 0, abort_flag = 1;
         return __shfl_sync(0xffffffffu, ok, 0) != 0;
     };
     auto arrive = [&](uint32_t b) {  // once for the warp, after all its lanes
@@ -334,124 +353,136 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
     };
 
     const int64_t tile = ((int64_t)seq * p.pool.kv_heads + kvh) * p.row_tiles + rt;
-    // The ring's tiles in the order in which the products take them:
-    // K0, then V(j), K(j + 1) (SPLIT: K(j + 1), V(j): the scores of a tile are
-    // asked for before the output of the one before).
+    // The tiles in the order in which the products take them: K0, then V(j),
+    // K(j + 1) (SPLIT: K(j + 1), V(j): the scores of a tile are asked for before
+    // the output of the one before).
+    struct Item {
+        int j, k_done, v_done;  // key tile; K and V tiles up to and with this one
+        bool is_v;
+    };
+    auto after = [&](const Item &a) {
+        Item b;
+        b.is_v = SPLIT ? !(a.k_done < n && a.k_done < a.v_done + 2) : a.v_done < a.k_done;
+        b.j = b.is_v ? a.v_done : a.k_done;
+        b.k_done = a.k_done + !b.is_v, b.v_done = a.v_done + b.is_v;
+        return b;
+    };
     if (wg == 2) {
         // ---- codes to float16 tiles ----
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PreRegs<SPLIT>::convert));
-        constexpr int PER = kPreKeys * D / 16 / 128;  // 16-byte pieces of a tile that a thread takes: 8 or 4
-        constexpr int CPR = D / 16;                   // pieces of a row
-        constexpr int RSTEP = 128 / CPR;              // rows between a thread's pieces: 16 or 32
-        const int row0 = t / CPR, ch = t % CPR;
-        const int per_page = p.pool.page / kKv8Block;
-        const int64_t head_off = (int64_t)kvh * p.pool.page;
-        // Three tiles are under way, so that neither the table's nor the pages'
-        // latency is waited for: the page numbers of the one after next (lane b
-        // looks up block b: as `block` codes into the pool, -1 for none), the
-        // codes of the next, the conversion of this one.
-        struct Item {
-            int j, k_done, v_done;  // key tile; K and V tiles up to and with this one
-            bool is_v;
-        };
-        auto after = [&](const Item &a) {
-            Item b;
-            b.is_v = SPLIT ? !(a.k_done < n && a.k_done < a.v_done + 2) : a.v_done < a.k_done;
-            b.j = b.is_v ? a.v_done : a.k_done;
-            b.k_done = a.k_done + !b.is_v, b.v_done = a.v_done + b.is_v;
-            return b;
-        };
-        // row of the pool ([page][kv head][token]) where the lane's block starts, -1 for none
-        auto look = [&](const Item &a) -> int64_t {
-            const int key = k_lo + a.j * kPreKeys + (lane & (kPreBlocks - 1)) * kKv8Block;
-            if (a.j >= n || key >= k_hi) return -1;
-            const int blk = key / kKv8Block, lp = blk / per_page;
-            const int id = kv8_page(p.pool, s, lp);
-            if (id < 0) bad_flag = 1;
-            return id < 0 ? -1 : (int64_t)id * p.pool.kv_heads * p.pool.page + head_off + (blk - lp * per_page) * kKv8Block;
-        };
-        auto load = [&](const Item &a, int64_t at, uint4 (&raw)[PER], float &ks, float &vs) {
-            const uint8_t *codes = (a.is_v ? p.pool.v : p.pool.k) + (row0 % kKv8Block) * D + ch * 16;
-            const int key = k_lo + a.j * kPreKeys + row0;
-#pragma unroll
+        // A thread takes 16-byte pieces: piece ch of rows row0, row0 + RSTEP, ...
+        // Eight lanes that store together hold two rows of unlike parity and four
+        // pieces of one half, which the swizzle puts into different banks.
+        constexpr int PER = kPreKeys * D / 16 / 128;  // 8 (D = 128) or 4
+        constexpr int RSTEP = kPreKeys / PER;         // 16 or 32
+        const int row0 = D == 128 ? 4 * (warp & 3) + (lane >> 4) * 2 + ((lane >> 2) & 1) : t / 4;
+        const int ch = D == 128 ? (lane & 3) + 4 * ((lane >> 3) & 1) : t % 4;
+        const uint32_t st0 = tile_off(row0, 2 * ch), st1 = tile_off(row0, 2 * ch + 1);  // RSTEP rows: RSTEP * 128 bytes
+        Item item{0, 1, 0, false};
+        RingPos rp, rr;
+        for (int it = 0; it < 2 * n; it++) {
+            if (!wait_warp(bar(RF + rr.idx), rr.phase)) break;
+            if (rp.uses >= (uint32_t)kPreRing && !wait_warp(bar(EMPTY + rp.idx), rp.phase ^ 1u)) break;
+            const uint32_t dst = ring + rp.idx * TILE, src = raw + rr.idx * (TILE / 2) + (uint32_t)(row0 * D + ch * 16);
+            const int left = k_hi - (k_lo + item.j * kPreKeys) - row0;  // rows past the range are zeros
+#pragma unroll 2
             for (int k = 0; k < PER; k++) {
-                const int64_t r = __shfl_sync(0xffffffffu, at, (row0 + k * RSTEP) / kKv8Block);
-                const bool ok = r >= 0 && key + k * RSTEP < k_hi;
-                raw[k] = make_uint4(0, 0, 0, 0);
-                if (ok) raw[k] = __ldg(reinterpret_cast<const uint4 *>(codes + r * D));
+                uint4 c = lds128(src + (uint32_t)k * (RSTEP * D));
+                if (k * RSTEP >= left) c = make_uint4(0, 0, 0, 0);
+                uint32_t h[8];
+                codes_to_half<E4M3>(c, h);
+                sts128(dst + st0 + (uint32_t)k * (RSTEP * 128), h[0], h[1], h[2], h[3]);
+                sts128(dst + st1 + (uint32_t)k * (RSTEP * 128), h[4], h[5], h[6], h[7]);
             }
-            // lane b of the first warp: the scales of block b
-            ks = vs = 1.f;
-            if (warp == 8 && !a.is_v && at >= 0) ks = p.pool.ks[at / kKv8Block], vs = p.pool.vs[at / kKv8Block];
-        };
-        uint4 raw[2][PER];
-        float ks[2], vs[2];
-        Item item{0, 1, 0, false}, next = after(item);
-        load(item, look(item), raw[0], ks[0], vs[0]);
-        int64_t at = look(next);
-        RingPos rp;
-        bool ok = true;
-        for (int it = 0; it < 2 * n && ok; it += 2) {
-#pragma unroll
-            for (int x = 0; x < 2; x++) {  // 2 n tiles: an even number
-                load(next, at, raw[x ^ 1], ks[x ^ 1], vs[x ^ 1]);
-                const Item later = after(next);
-                at = look(later);
-                ok = ok && (rp.uses < (uint32_t)kPreRing || wait_warp(bar(EMPTY + rp.idx), rp.phase ^ 1u));
-                if (!ok) break;
-                const uint32_t dst = ring + rp.idx * TILE;
-#pragma unroll
-                for (int k = 0; k < PER; k++) {
-                    uint32_t h[8];
-                    codes_to_half<E4M3>(raw[x][k], h);
-                    const int row = row0 + k * RSTEP;
-                    const uint32_t a = dst + tile_off(row, 2 * ch), b = dst + tile_off(row, 2 * ch + 1);
-                    // eight lanes of one row: pieces of both halves fall into different banks
-                    const bool odd = ch >= 4;
-                    sts128(odd ? b : a, odd ? h[4] : h[0], odd ? h[5] : h[1], odd ? h[6] : h[2], odd ? h[7] : h[3]);
-                    sts128(odd ? a : b, odd ? h[0] : h[4], odd ? h[1] : h[5], odd ? h[2] : h[6], odd ? h[3] : h[7]);
-                }
-                if (warp == 8 && lane < kPreBlocks && !item.is_v) {
-                    scales[item.j & 3][0][lane] = ks[x];
-                    scales[item.j & 3][1][lane] = __log2f(vs[x]);
-                    scales[item.j & 3][2][lane] = 1.f / vs[x];
-                }
-                fence_async();
-                arrive(bar(FULL + rp.idx));
-                rp.next(kPreRing);
-                item = next;
-                next = later;
-            }
+            fence_async();
+            arrive(bar(FULL + rp.idx));
+            if (lane == 0) mbar_arrive(bar(RE + rr.idx));
+            rp.next(kPreRing);
+            rr.next(kPreRaw);
+            item = after(item);
         }
     } else if (wg == 3) {
         // ---- the products ----
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PreRegs<SPLIT>::issue));
-        if (warp == 12 && lane == 0 && n > 0) {
+        if (warp == 13 && n > 0) {
+            // the tiles' pages: lane b takes block b
+            const uint32_t per_page = (uint32_t)(p.pool.page / kKv8Block);
+            // The block of the layer's pool ([page][kv head][block]): 0 past the range
+            // and, with bad_flag, for a page out of range.  (Below 2^31: a pool of
+            // that many blocks would be 2 TB.)
+            auto look = [&](int j) -> uint32_t {
+                const int key = k_lo + j * kPreKeys + lane * kKv8Block;
+                if (lane >= kPreBlocks || j >= n || key >= k_hi) return 0;
+                const uint32_t blk = (uint32_t)key / kKv8Block, lp = blk / per_page;
+                const int id = kv8_page(p.pool, s, (int)lp);
+                if (id < 0) bad_flag = 1;
+                return id < 0 ? 0u : ((uint32_t)id * (uint32_t)p.pool.kv_heads + (uint32_t)kvh) * per_page + (blk - lp * per_page);
+            };
+            Item item{0, 1, 0, false};
+            uint32_t at = look(0);
+            RingPos rr;
+            for (int it = 0; it < 2 * n; it++) {
+                const Item next = after(item);
+                const uint32_t at_next = look(next.j);  // looked up while this tile's slot is waited for
+                const int left = k_hi - (k_lo + item.j * kPreKeys);
+                const int blocks = min((left + kKv8Block - 1) / kKv8Block, kPreBlocks);
+                float ks = 1.f, vs = 1.f;
+                if (!item.is_v && lane < blocks) ks = p.pool.ks[at], vs = p.pool.vs[at];
+                if (rr.uses >= (uint32_t)kPreRaw && !wait_warp(bar(RE + rr.idx), rr.phase ^ 1u)) break;
+                if (!item.is_v && lane < kPreBlocks) {
+                    scales[item.j & 7][0][lane] = ks;
+                    scales[item.j & 7][1][lane] = __log2f(vs);
+                    scales[item.j & 7][2][lane] = 1.f / vs;
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive_expect_tx(bar(RF + rr.idx), (uint32_t)blocks * (kKv8Block * D));
+                __syncwarp();
+                if (lane < blocks)
+                    bulk_g2s(raw + rr.idx * (TILE / 2) + (uint32_t)lane * (kKv8Block * D),
+                             (item.is_v ? p.pool.v : p.pool.k) + (uint64_t)at * (kKv8Block * D), kKv8Block * D,
+                             bar(RF + rr.idx));
+                rr.next(kPreRaw);
+                item = next;
+                at = at_next;
+            }
+            // every copy has landed before the block ends
+            if (lane == 0)
+                for (uint32_t i = 0; i < (uint32_t)kPreRaw; i++) {
+                    const uint32_t uses = rr.uses / kPreRaw + (i < rr.uses % kPreRaw ? 1u : 0u);
+                    if (uses) poll(bar(RF + i), (uses - 1) & 1u);
+                }
+            __syncwarp();
+        } else if (warp == 12 && n > 0) {
             constexpr uint32_t IQK = idesc_f16(kPreKeys, false), IPV = idesc_f16(D, true);
+            constexpr uint32_t HI = desc_hi(1024);  // eight rows of 128 bytes
+            const uint32_t one = lane == 0;
             RingPos rp;
             bool ok = true;
             auto take = [&](uint32_t &slot) {
                 slot = rp.idx;
-                ok = ok && wait(bar(FULL + rp.idx), rp.phase);
+                ok = ok && wait_warp(bar(FULL + rp.idx), rp.phase);
                 fence_after();
                 rp.next(kPreRing);
             };
             // scores = q tile x K; K-major both: 16 values are 32 bytes into a 128-byte row
             auto qk = [&](uint32_t d, uint32_t q, uint32_t slot, bool acc) {
-                const uint64_t da = smem_desc_sw128(q, 16u, 1024u), db = smem_desc_sw128(ring + slot * TILE, 16u, 1024u);
-#pragma unroll 1
+                const uint32_t da = desc_lo(q, 16u), db = desc_lo(ring + slot * TILE, 16u);
+#pragma unroll
                 for (int k = 0; k < D / 16; k++) {
-                    const uint64_t off = (uint64_t)(((k >> 2) * HALF + (k & 3) * 32u) >> 4);
-                    umma_f16(d, da + off, db + off, IQK, (k > 0 || acc) ? 1u : 0u);
+                    const uint32_t off = ((k >> 2) * HALF + (k & 3) * 32u) >> 4;
+                    umma_f16(d, da + off, db + off, HI, IQK, (k > 0 || acc) ? 1u : 0u, one);
                 }
             };
-            // output = e x V; e: 16 keys are 8 of every 32 columns' first 16; V N-major: 16 keys are 2048 bytes, the next 64 values HALF further
+            // output = e x V; e: 16 keys are 8 of every 32 columns' first 16; V N-major: 16 keys
+            // are 2048 bytes, the next 64 values HALF further
             auto pv = [&](uint32_t d, uint32_t e, uint32_t slot, bool acc) {
-                const uint64_t db = smem_desc_sw128(ring + slot * TILE, HALF, 1024u);
-#pragma unroll 1
+                const uint32_t db = desc_lo(ring + slot * TILE, HALF);
+#pragma unroll
                 for (int k = 0; k < kPreKeys / 16; k++)
-                    umma_f16_ts(d, e + 32u * (k >> 1) + 8u * (k & 1), db + (uint64_t)(k * 2048u >> 4), IPV, (k > 0 || acc) ? 1u : 0u);
+                    umma_f16_ts(d, e + 32u * (k >> 1) + 8u * (k & 1), db + (k * 2048u >> 4), HI, IPV,
+                                (k > 0 || acc) ? 1u : 0u, one);
             };
+            auto commit = [&](uint32_t b) { umma_commit_one(b, one); };
             uint32_t ks, vs;
             if constexpr (SPLIT) {
                 auto scores = [&](int j) {
@@ -460,75 +491,74 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
                     const uint32_t d = tmem + kS + 128u * (j & 1);
                     qk(d, q_tile, ks, false);
                     qk(d, q_tile + TILE, ks, true);
-                    umma_commit(bar(SF + (j & 1)));
-                    umma_commit(bar(EMPTY + ks));
+                    commit(bar(SF + (j & 1)));
+                    commit(bar(EMPTY + ks));
                 };
                 scores(0);
                 if (ok && n > 1) scores(1);
                 for (int j = 0; j < n && ok; j++) {
                     const uint32_t b = j & 1, ph = (j >> 1) & 1;
                     take(vs);
-                    if (ok && j >= 2) ok = wait(bar(TE + b), ph ^ 1u);
-                    if (ok) ok = wait(bar(PF + b), ph);
+                    if (ok && j >= 2) ok = wait_warp(bar(TE + b), ph ^ 1u);
+                    if (ok) ok = wait_warp(bar(PF + b), ph);
                     if (!ok) break;
                     fence_after();
                     const uint32_t d = tmem + kO + 128u * b, e = tmem + kS + 128u * b;
                     pv(d, e, vs, false);
                     pv(d, e + 16u, vs, true);
-                    umma_commit(bar(TF + b));
-                    umma_commit(bar(EMPTY + vs));
+                    commit(bar(TF + b));
+                    commit(bar(EMPTY + vs));
                     if (j + 2 < n) scores(j + 2);
                 }
             } else {
                 take(ks);
                 if (ok) {
                     qk(tmem + kS, q_tile, ks, false);
-                    umma_commit(bar(SF));
+                    commit(bar(SF));
                     if (two) {
                         qk(tmem + kS + 128u, q_tile + TILE, ks, false);
-                        umma_commit(bar(SF + 1));
+                        commit(bar(SF + 1));
                     }
-                    umma_commit(bar(EMPTY + ks));
+                    commit(bar(EMPTY + ks));
                 }
                 for (int j = 0; j < n && ok; j++) {
                     const uint32_t ph = j & 1;
                     const bool more = j + 1 < n;
                     take(vs);
-                    if (ok) ok = wait(bar(PF), ph);
+                    if (ok) ok = wait_warp(bar(PF), ph);
                     if (!ok) break;
                     fence_after();
                     pv(tmem + kO, tmem + kS, vs, j > 0);
-                    if (!two) umma_commit(bar(EMPTY + vs));
+                    if (!two) commit(bar(EMPTY + vs));
                     if (more) {
                         take(ks);
                         if (!ok) break;
                         qk(tmem + kS, q_tile, ks, false);
-                        umma_commit(bar(SF));
-                        if (!two) umma_commit(bar(EMPTY + ks));
+                        commit(bar(SF));
+                        if (!two) commit(bar(EMPTY + ks));
                     } else {
-                        umma_commit(bar(TF));
+                        commit(bar(TF));
                     }
                     if (two) {
-                        ok = wait(bar(PF + 1), ph);
+                        ok = wait_warp(bar(PF + 1), ph);
                         if (!ok) break;
                         fence_after();
                         pv(tmem + kO + 128u, tmem + kS + 128u, vs, j > 0);
-                        umma_commit(bar(EMPTY + vs));
+                        commit(bar(EMPTY + vs));
                         if (more) {
                             qk(tmem + kS + 128u, q_tile + TILE, ks, false);
-                            umma_commit(bar(SF + 1));
-                            umma_commit(bar(EMPTY + ks));
+                            commit(bar(SF + 1));
+                            commit(bar(EMPTY + ks));
                         } else {
-                            umma_commit(bar(TF + 1));
+                            commit(bar(TF + 1));
                         }
                     }
                 }
             }
             // every product issued has finished before TMEM is given back
-            umma_commit(bar(DR));
-            if (!mbar_wait_bounded(bar(DR), 0, kPreWaitNs)) atomicExch(&g_kv8_prefill_status, kStatusTimeout);
+            commit(bar(DR));
+            wait_warp(bar(DR), 0);
         }
-        __syncwarp();
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PreRegs<SPLIT>::score));
         const uint32_t my = tmem + ((uint32_t)(32 * (warp & 3)) << 16);  // the warp's lanes
@@ -556,6 +586,11 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
         const float nan = __int_as_float(0x7fc00000);
         if (wg == 0 || (!SPLIT && two)) {
             // ---- scores to e ----
+            const bool there = r0 + row < rows_all;
+            const int ps = pos0 + (there ? (r0 + row) / p.g : 0);  // the row's position; it sees [see_lo, see_hi)
+            const int see_hi = !there ? 0 : min(p.causal ? ps + 1 : s.len, k_hi);
+            const int see_lo = p.window > 0 ? ps - p.window + 1 : 0;
+            const float rf = row_f[row];
             float m = -INFINITY, l = 0.f;
             const int warp_hi = __reduce_min_sync(0xffffffffu, see_hi), warp_lo = __reduce_max_sync(0xffffffffu, see_lo);
             bool ok = true;
@@ -568,7 +603,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
                 const uint32_t sc = my + kS + 128u * b;
                 const int key = k_lo + j * kPreKeys;
                 const bool edge = key < warp_lo || key + kPreKeys > warp_hi;
-                const float *kss = scales[j & 3][0], *lvs = scales[j & 3][1], *inv = scales[j & 3][2];
+                const float *kss = scales[j & 7][0], *lvs = scales[j & 7][1], *inv = scales[j & 7][2];
                 // 32 scores (two blocks) at a time, twice: rolled loops, because the
                 // roles' code has to stay in the instruction cache together
                 uint32_t x[32];
@@ -589,11 +624,16 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
                     scores(i);
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        float a = __uint_as_float(x[16 * h]);
+                        float a[4];
 #pragma unroll
-                        for (int u = 1; u < kKv8Block; u++) a = fmaxf(a, __uint_as_float(x[16 * h + u]));
+                        for (int u = 0; u < 4; u++) {  // short chains: four at a time
+                            const uint32_t *y = x + 16 * h + 4 * u;
+                            a[u] = fmaxf(fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1])),
+                                         fmaxf(__uint_as_float(y[2]), __uint_as_float(y[3])));
+                        }
+                        const float top = fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3]));
                         // the factor above 0: -inf stays -inf
-                        mx = fmaxf(mx, fmaf(a, fmaxf(kss[2 * i + h] * rf, 1.4e-45f), lvs[2 * i + h]));
+                        mx = fmaxf(mx, fmaf(top, fmaxf(kss[2 * i + h] * rf, 1.4e-45f), lvs[2 * i + h]));
                     }
                 }
                 float al = 1.f;
@@ -631,19 +671,21 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
                         const float kf = fmaxf(kss[2 * i + h] * rf, 1.4e-45f), d = lvs[2 * i + h] - off;
-                        float sum = 0.f;
+                        const float2 kf2 = make_float2(kf, kf), d2 = make_float2(d, d);
+                        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-                        for (int u = 0; u < kKv8Block; u++) {
-                            const float e = ex2p(fmaf(__uint_as_float(x[16 * h + u]), kf, d));
-                            sum += e;
-                            x[16 * h + u] = __float_as_uint(e);
+                        for (int u = 0; u < 8; u++) {
+                            uint32_t *y = x + 16 * h + 2 * u;
+                            float2 e = f2fma(make_float2(__uint_as_float(y[0]), __uint_as_float(y[1])), kf2, d2);
+                            e.x = ex2p(e.x), e.y = ex2p(e.y);
+                            sum[u & 1] = f2add(sum[u & 1], e);
+                            y[0] = __float_as_uint(e.x), y[1] = __float_as_uint(e.y);
+                            hp[8 * h + u] = pack_half(e.x, e.y);
                         }
-                        l = fmaf(sum, inv[2 * i + h], l);
+                        sum[0] = f2add(sum[0], sum[1]);
+                        l = fmaf(sum[0].x + sum[0].y, inv[2 * i + h], l);
                     }
                     // e as float16 over its scores: 16 columns (SPLIT: the low parts in the 16 after)
-#pragma unroll
-                    for (int u = 0; u < 16; u++)
-                        hp[u] = pack_half(__uint_as_float(x[2 * u]), __uint_as_float(x[2 * u + 1]));
                     tmem_st16(sc + 32u * i, hp);
                     if constexpr (SPLIT) {
 #pragma unroll
@@ -729,6 +771,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
     }
     if (tid == 0) {
         if (bad_flag) atomicExch(&g_kv8_prefill_status, VKQ_ERR_INVALID_ARGUMENT);
+        if (abort_flag) atomicExch(&g_kv8_prefill_status, kStatusTimeout);
         last = active > 1 && atomicAdd(p.count + tile, 1u) == (unsigned)active - 1u;
     }
     __syncthreads();
@@ -817,7 +860,7 @@ cudaError_t kv8_prefill(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_bat
     const void *fn = a.dtype == VKQ_F32   ? prefill_fn<float>(c.head_dim, p.pool.e4m3)
                      : a.dtype == VKQ_F16 ? prefill_fn<__half>(c.head_dim, p.pool.e4m3)
                                           : prefill_fn<__nv_bfloat16>(c.head_dim, p.pool.e4m3);
-    const size_t smem = (size_t)(2 + kPreRing) * 128 * c.head_dim * 2 + 1024;
+    const size_t smem = (size_t)((2 + kPreRing) * 2 + kPreRaw) * 128 * c.head_dim + 1024;
     cudaError_t e = kernel_smem(fn, smem, true);
     if (e != cudaSuccess) return e;
     // the warpgroups' register split draws on what the block is launched with
