@@ -57,17 +57,18 @@ struct Kv8Seq {
 
 __device__ __forceinline__ Kv8Seq kv8_seq(const Kv8Batch &b, int page, int64_t i) {
     Kv8Seq s{};
+    // all loads first (the row clamped for the length's), then the checks
     const int64_t c0 = b.cu ? b.cu[i] : i, c1 = b.cu ? b.cu[i + 1] : i + 1;
+    const int64_t r = b.slots ? b.slots[i] : i;
+    const int64_t in = r < 0 ? 0 : r < b.rows ? r : b.rows - 1;
+    const int len = b.lens[in];
     s.ok = c0 >= 0 && c1 >= c0 && c1 <= b.tokens && c1 - c0 <= b.max_tokens;
     if (!s.ok) return s;  // n == 0: no rows of this sequence are known
     s.first = (int)c0;
     s.n = (int)(c1 - c0);
-    const int64_t r = b.slots ? b.slots[i] : i;
-    s.ok = r >= 0 && r < b.rows;
-    if (!s.ok) return s;
-    s.pages = b.table + r * b.max_pages;
-    s.len = b.lens[r];
-    s.ok = s.len >= 0 && s.len <= b.max_len && s.len <= b.max_pages * page;
+    s.ok = r == in && len >= 0 && len <= b.max_len && len <= b.max_pages * page;
+    s.pages = b.table + in * b.max_pages;
+    s.len = len;
     return s;
 }
 
@@ -75,6 +76,15 @@ __device__ __forceinline__ Kv8Seq kv8_seq(const Kv8Batch &b, int page, int64_t i
 __device__ __forceinline__ int kv8_page(const Kv8Pool &p, const Kv8Seq &s, int lp) {
     const int id = s.pages[lp];
     return id >= 0 && id < p.num_pages ? id : -1;
+}
+
+// x / d for d >= 1 by a multiplication: `magic` is floor((2^32 - 1) / d) + 1 (0
+// for d = 1), the quotient then at most one too large.
+inline uint32_t kv8_magic(uint32_t d) { return d == 1 ? 0u : 0xffffffffu / d + 1u; }
+__device__ __forceinline__ uint32_t kv8_div(uint32_t x, uint32_t d, uint32_t magic) {
+    uint32_t q = magic ? __umulhi(x, magic) : x;
+    if (q * d > x) q--;
+    return q;
 }
 
 // ---- codes ----------------------------------------------------------------
@@ -100,6 +110,25 @@ __device__ __forceinline__ float kv8_scale(float a, bool e4m3) {
     float s = __uint_as_float((uint32_t)(max(e, -126) + 127) << 23);
     if (a > m * s) s *= 2.f;
     return fminf(fmaxf(s, kKv8MinScale), kKv8MaxScale);
+}
+
+// Codes as float16 pairs, exactly.  int8: the byte with its sign bit flipped
+// (kv8_unsign) is the low byte of 1024 + 128 + code.  e4m3: the hardware's
+// conversion (0x7f and 0xff, which are no codes, give NaN).
+template <bool E4M3> __device__ __forceinline__ uint32_t kv8_unsign(uint32_t w) { return E4M3 ? w : w ^ 0x80808080u; }
+// Bytes (0, 1) or (2, 3) of an unsigned word.
+template <bool E4M3, bool HIGH>
+__device__ __forceinline__ uint32_t kv8_widen(uint32_t w) {
+    if constexpr (E4M3) {
+        uint32_t r;
+        if constexpr (HIGH) asm("{ .reg .b16 a, b; mov.b32 {a, b}, %1; cvt.rn.f16x2.e4m3x2 %0, b; }" : "=r"(r) : "r"(w));
+        else asm("{ .reg .b16 a, b; mov.b32 {a, b}, %1; cvt.rn.f16x2.e4m3x2 %0, a; }" : "=r"(r) : "r"(w));
+        return r;
+    } else {
+        const uint32_t u = prmt(w, 0x64646464u, HIGH ? 0x4342u : 0x4140u);
+        const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&u), __half2half2(__ushort_as_half(0x6480)));
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
 }
 
 }  // namespace vkq

@@ -14,8 +14,7 @@
 // order, so results do not depend on timing.
 //
 // The products run on m16n8k16 with float16 operands: codes are exact in
-// float16 (the conversion is two byte permutes and an add a pair), and a
-// decode step has at most 16 rows, where the 128-row tcgen05 tile would be
+// float16 (kv8_widen), and a decode step has at most 16 rows, where the 128-row tcgen05 tile would be
 // nearly empty.  Each lane's operand columns are chosen so that its 16-byte
 // loads from shared memory hold whole fragments: column k of a K step is
 // dimension 16 (c + 4 h) + 4 w + ..., column n of a V tile t is dimension
@@ -25,9 +24,9 @@
 // (22 bits), one product each: with 8 rows the parts are rows r and r + 8 of
 // one instruction, so the split costs nothing there.  q is first scaled by a
 // power of two of its row, and p by 2^14, to keep the low parts out of
-// float16's subnormals.  16-bit q is exact in float16 after that scaling, and
-// p is rounded once to 11 bits (2^-11, no more than the output's own rounding);
-// the tile then has 16 rows.  Each 16-key product starts from zero and is
+// float16's subnormals.  16-bit q is exact in float16 after that scaling; with
+// more than 8 rows its p is rounded once to 11 bits (2^-11, no more than the
+// output's own rounding) and the tile has 16 rows.  Each 16-key product starts from zero and is
 // added to the output in float32 with its vs: the accumulators of the matrix
 // unit round toward zero, which would add up over a long cache.
 #include <cmath>
@@ -46,7 +45,9 @@ static __device__ int g_kv8_attn_status;
 constexpr int kDecWarps = 4;
 constexpr int kDecThreads = 32 * kDecWarps;
 constexpr int kDecStep = 32;   // keys of a step: two scale blocks
-constexpr int kDecStages = 3;  // ring slots of a warp: two steps in flight
+constexpr int kDecStages = 2;  // ring slots of a warp
+// CTAs an SM that registers and rings are cut for (16 rows take the registers of two)
+constexpr int dec_ctas(int rows) { return rows == 8 ? 3 : 2; }
 
 struct DecodeParams {
     Kv8Pool pool;
@@ -55,6 +56,7 @@ struct DecodeParams {
     void *out;
     int64_t qt, ot;
     int heads, g, row_tiles, splits, chunk;
+    uint32_t magic;  // of page / 16 (kv8_div)
     float f;      // scale * log2(e)
     int causal, window;
     bool vec;     // rows of q and out are 16-byte aligned
@@ -80,22 +82,19 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-
-// Bytes (0, 1) or (2, 3) of w as a float16 pair.  int8: the byte with its sign
-// bit flipped is the low byte of 1024 + 128 + code; e4m3: its bits are those
-// of a float16 2^8 too small (exponent bias 7 against 15), subnormals included.
-template <bool E4M3, bool HIGH>
-__device__ __forceinline__ uint32_t widen(uint32_t w) {
-    if constexpr (E4M3) {
-        const uint32_t h = prmt(w, 0u, HIGH ? 0x3424u : 0x1404u);
-        return (h & 0x80008000u) | ((h >> 1) & 0x3F803F80u);
-    } else {
-        const uint32_t u = prmt(w, 0x64646464u, HIGH ? 0x4342u : 0x4140u);
-        const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&u), __half2half2(__ushort_as_half(0x6480)));
-        return *reinterpret_cast<const uint32_t *>(&h);
-    }
+// The same from zero.
+__device__ __forceinline__ void mma_f16_new(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
-template <bool E4M3> __device__ __forceinline__ uint32_t unsign(uint32_t w) { return E4M3 ? w : w ^ 0x80808080u; }
+
+// The sum over a warp's lanes, the same in each.
+__device__ __forceinline__ float warp_total(float s) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    return s;
+}
 
 // Byte offset of 16-byte piece `ch` of row r (of 16) in a ring slot, permuted
 // so that the K reads (two rows, four pieces) and the V reads (four even or
@@ -106,10 +105,13 @@ __device__ __forceinline__ uint32_t slot_off(int r, int ch) {
     else return (uint32_t)((r >> 1) * 128 + (((((r & 1) << 2) | ch) ^ (((r >> 1) & 3) << 1)) << 4));
 }
 
-template <typename T, int D, bool E4M3>
-__global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const DecodeParams p) {
-    constexpr bool SPLIT = sizeof(T) == 4;
-    constexpr int ROWS = SPLIT ? 8 : 16, NR = SPLIT ? 1 : 2;  // rows of a tile, rows of a lane
+template <typename T, int D, bool E4M3, int ROWS>
+__global__ void __launch_bounds__(kDecThreads, dec_ctas(ROWS)) kv8_decode_kernel(const DecodeParams p) {
+    // Eight rows leave the instruction's other eight to the low parts (of 16-bit
+    // q: zeros); sixteen 16-bit rows are rounded.
+    constexpr bool SPLIT = ROWS == 8;
+    static_assert(SPLIT || sizeof(T) == 2, "float32 takes both parts");
+    constexpr int NR = ROWS / 8;  // rows of a lane
     constexpr int KS = D / 16;                                // K steps
     constexpr int NT = D / 8;                                 // V tiles
     constexpr int UNIT = kKv8Block * D;                       // code bytes of 16 keys
@@ -145,6 +147,56 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const DecodePar
     if (split >= active) return;
     const int k_lo = lo + split * p.chunk, k_hi = min(hi, k_lo + p.chunk);
 
+    // the warp's ring
+    const uint32_t my_ring = smem_u32addr(ring) + (uint32_t)(warp * kDecStages * SLOT);
+    const int steps = k_hi > k_lo ? (k_hi - k_lo + kDecStep - 1) / kDecStep : 0;
+    const int mine = steps > warp ? (steps - warp + kDecWarps - 1) / kDecWarps : 0;
+    bool bad = false;
+    const uint32_t per_page = (uint32_t)(p.pool.page / kKv8Block);
+    const int lrow = lane / (D / 16), lch = lane % (D / 16);   // the lane's first piece; the next are LSTEP rows on
+    constexpr int LSTEP = 32 / (D / 16), PIECES = UNIT / 512;  // 4 rows, 4 pieces (D = 64: 8, 2)
+    uint32_t loff[PIECES];
+#pragma unroll
+    for (int i = 0; i < PIECES; i++) loff[i] = slot_off<D>(lrow + i * LSTEP, lch);
+    auto fill = [&](int it) {
+        if (it < mine) {
+            const uint32_t slot = my_ring + (uint32_t)(it % kDecStages) * SLOT;
+            const int key = k_lo + (warp + it * kDecWarps) * kDecStep;
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int k0 = key + u * kKv8Block;
+                // the unit's block in the layer's pool ([page][kv head][block]), 0 where there is none
+                int id = -1;
+                uint32_t blk = (uint32_t)k0 / kKv8Block;
+                if (k0 < k_hi) {
+                    const uint32_t lp = kv8_div(blk, per_page, p.magic);
+                    id = kv8_page(p.pool, s, (int)lp);
+                    bad |= id < 0;
+                    blk -= lp * per_page;
+                }
+                const int rows = id < 0 ? 0 : min(k_hi - k0, kKv8Block);
+                const int64_t b = id < 0 ? 0 : ((int64_t)id * p.pool.kv_heads + kvh) * per_page + blk;
+                const uint8_t *ks = p.pool.k + b * UNIT + lane * 16, *vs = p.pool.v + b * UNIT + lane * 16;
+                const uint32_t kd = slot + (uint32_t)(u * UNIT), vd = slot + (uint32_t)((2 + u) * UNIT);
+#pragma unroll
+                for (int i = 0; i < PIECES; i++) {  // rows past the range are zeros
+                    const uint32_t bytes = lrow + i * LSTEP < rows ? 16u : 0u;
+                    cp_async16(kd + loff[i], ks + i * 512, bytes);
+                    cp_async16(vd + loff[i], vs + i * 512, bytes);
+                }
+                if (lane < 2)
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(slot + 4u * UNIT + 8u * u + 4u * lane),
+                                 "l"((lane ? p.pool.vs : p.pool.ks) + b), "r"(id < 0 ? 0u : 4u)
+                                 : "memory");
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+
+    // the first steps are under way while q is loaded
+#pragma unroll
+    for (int it = 0; it < kDecStages - 1; it++) fill(it);
+
     // q: the lane's rows (n8, and n8 + 8 with 16-bit rows), scaled to below 2^15
     uint32_t qa[KS][4];
     float rf[NR];          // what a score of the row is multiplied by, with ks
@@ -170,7 +222,7 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const DecodePar
         a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
         const int e = min(max((int)(__float_as_uint(a) >> 23) - 127, -60), 127);
         const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
-        rf[u] = p.f * __uint_as_float((uint32_t)(e - 14 + 127) << 23) * (E4M3 ? 256.f : 1.f);
+        rf[u] = p.f * __uint_as_float((uint32_t)(e - 14 + 127) << 23);
 #pragma unroll
         for (int hh = 0; hh < D / 64; hh++)
 #pragma unroll
@@ -189,47 +241,6 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const DecodePar
                 }
     }
 
-    // the warp's ring
-    const uint32_t my_ring = smem_u32addr(ring) + (uint32_t)(warp * kDecStages * SLOT);
-    const int steps = k_hi > k_lo ? (k_hi - k_lo + kDecStep - 1) / kDecStep : 0;
-    const int mine = steps > warp ? (steps - warp + kDecWarps - 1) / kDecWarps : 0;
-    bool bad = false;
-    auto fill = [&](int it) {
-        if (it < mine) {
-            const uint32_t slot = my_ring + (uint32_t)(it % kDecStages) * SLOT;
-            const int key = k_lo + (warp + it * kDecWarps) * kDecStep;
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const int k0 = key + u * kKv8Block;
-                int id = -1;
-                if (k0 < k_hi) {
-                    id = kv8_page(p.pool, s, k0 / p.pool.page);
-                    bad |= id < 0;
-                }
-                const int in_page = k0 % p.pool.page;
-                const int64_t ph = (int64_t)max(id, 0) * p.pool.kv_heads + kvh;
-                const int64_t at = (ph * p.pool.page + in_page) * D;
-                const int rows = id < 0 ? 0 : k_hi - k0;
-#pragma unroll
-                for (int i = lane; i < UNIT / 16; i += 32) {
-                    const int r = i / (D / 16), ch = i % (D / 16);
-                    const uint32_t bytes = r < rows ? 16u : 0u;
-                    const int64_t e = bytes ? at + i * 16 : 0;
-                    cp_async16(slot + (uint32_t)(u * UNIT) + slot_off<D>(r, ch), p.pool.k + e, bytes);
-                    cp_async16(slot + (uint32_t)((2 + u) * UNIT) + slot_off<D>(r, ch), p.pool.v + e, bytes);
-                }
-                if (lane < 2) {
-                    const float *sc = lane ? p.pool.vs : p.pool.ks;
-                    const int64_t e = id < 0 ? 0 : ph * (p.pool.page / kKv8Block) + in_page / kKv8Block;
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(slot + 4u * UNIT + 8u * u + 4u * lane),
-                                 "l"(sc + e), "r"(id < 0 ? 0u : 4u)
-                                 : "memory");
-                }
-            }
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-
     float m[NR], l[NR];
     float2 o[NT][NR];
 #pragma unroll
@@ -239,12 +250,10 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const DecodePar
 #pragma unroll
         for (int t = 0; t < NT; t++) o[t][u] = make_float2(0.f, 0.f);
     }
-#pragma unroll
-    for (int it = 0; it < kDecStages - 1; it++) fill(it);
     for (int it = 0; it < mine; it++) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kDecStages - 2) : "memory");
-        __syncwarp();
         fill(it + kDecStages - 1);  // into the slot read one pass ago
+        asm volatile("cp.async.wait_group %0;" ::"n"(kDecStages - 1) : "memory");
+        __syncwarp();
         const uint32_t slot = my_ring + (uint32_t)(it % kDecStages) * SLOT;
         const int key = k_lo + (warp + it * kDecWarps) * kDecStep;
         const uint4 scw = lds128(slot + 4u * UNIT);  // ks, vs of unit 0; of unit 1
@@ -256,15 +265,16 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const DecodePar
         for (int u = 0; u < 2; u++)
 #pragma unroll
             for (int t = 0; t < 2; t++) {
-                float d[4] = {0.f, 0.f, 0.f, 0.f};
+                float d[4];
 #pragma unroll
                 for (int hh = 0; hh < D / 64; hh++) {
                     const uint4 kw = lds128(slot + (uint32_t)(u * UNIT) + slot_off<D>(8 * t + n8, c + 4 * hh));
                     const uint32_t w[4] = {kw.x, kw.y, kw.z, kw.w};
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const uint32_t b = unsign<E4M3>(w[i]);
-                        mma_f16(d, qa[4 * hh + i], widen<E4M3, false>(b), widen<E4M3, true>(b));
+                        const uint32_t b = kv8_unsign<E4M3>(w[i]);
+                        if (hh == 0 && i == 0) mma_f16_new(d, qa[0], kv8_widen<E4M3, false>(b), kv8_widen<E4M3, true>(b));
+                        else mma_f16(d, qa[4 * hh + i], kv8_widen<E4M3, false>(b), kv8_widen<E4M3, true>(b));
                     }
                 }
                 const int j = key + u * kKv8Block + 8 * t + 2 * c;
@@ -330,7 +340,7 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const DecodePar
                     pa[2 * t + 1] = half2_bits(x[u][t][NR - 1][0], x[u][t][NR - 1][1]);
                 }
             }
-            const float sc = vs[u] * (E4M3 ? 256.f : 1.f);
+            const float sc = vs[u];
             const float2 sc2 = make_float2(sc, sc);
             const uint32_t vb = slot + (uint32_t)((2 + u) * UNIT);
             uint32_t w[4][NT / 4];  // the lane's dimensions of keys 2c, 2c + 1, 2c + 8, 2c + 9
@@ -349,13 +359,13 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const DecodePar
             for (int i = 0; i < NT / 4; i++)
 #pragma unroll
                 for (int z = 0; z < 2; z++) {  // dimensions 4i + 2z, + 1: bytes of two keys side by side
-                    const uint32_t b0 = unsign<E4M3>(prmt(w[0][i], w[1][i], z ? 0x7362u : 0x5140u));
-                    const uint32_t b1 = unsign<E4M3>(prmt(w[2][i], w[3][i], z ? 0x7362u : 0x5140u));
+                    const uint32_t b0 = kv8_unsign<E4M3>(prmt(w[0][i], w[1][i], z ? 0x7362u : 0x5140u));
+                    const uint32_t b1 = kv8_unsign<E4M3>(prmt(w[2][i], w[3][i], z ? 0x7362u : 0x5140u));
 #pragma unroll
                     for (int y = 0; y < 2; y++) {
-                        float d[4] = {0.f, 0.f, 0.f, 0.f};
-                        if (y == 0) mma_f16(d, pa, widen<E4M3, false>(b0), widen<E4M3, false>(b1));
-                        else mma_f16(d, pa, widen<E4M3, true>(b0), widen<E4M3, true>(b1));
+                        float d[4];
+                        if (y == 0) mma_f16_new(d, pa, kv8_widen<E4M3, false>(b0), kv8_widen<E4M3, false>(b1));
+                        else mma_f16_new(d, pa, kv8_widen<E4M3, true>(b0), kv8_widen<E4M3, true>(b1));
                         const int t = 4 * i + 2 * z + y;
                         if constexpr (SPLIT) {
                             o[t][0] = f2fma(f2add(make_float2(d[0], d[1]), make_float2(d[2], d[3])), sc2, o[t][0]);
@@ -429,43 +439,58 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const DecodePar
     if (threadIdx.x == 0) p.count[tile] = 0;
     part = p.part + tile * p.splits * ROWS * D;
     stat = p.stat + tile * p.splits * ROWS * 2;
+    // each range's weight for each row, 1 / l folded in; then the sums, many loads in flight
+    float *wt = reinterpret_cast<float *>(ring);  // [range][row]
+    for (int r = warp; r < ROWS; r += kDecWarps) {
+        float mx = -INFINITY, sum = 0.f;
+        for (int w = lane; w < active; w += 32) mx = fmaxf(mx, __ldcg(stat + (w * ROWS + r) * 2));
+#pragma unroll
+        for (int i = 16; i > 0; i >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, i));
+        for (int w = lane; w < active; w += 32) {
+            const float2 ms = __ldcg(reinterpret_cast<const float2 *>(stat + (w * ROWS + r) * 2));
+            const float k = ms.x == -INFINITY ? 0.f : ex2(ms.x - mx);
+            sum += k * ms.y;
+            wt[w * ROWS + r] = k;
+        }
+        sum = warp_total(sum);
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        __syncwarp();
+        for (int w = lane; w < active; w += 32) wt[w * ROWS + r] *= inv;
+    }
+    __syncthreads();
     for (int i = threadIdx.x; i < ROWS * D / 4; i += kDecThreads) {
         const int r = i / (D / 4), d = i % (D / 4) * 4;
         if (r0 + r >= rows_all) continue;
-        float mx = -INFINITY;
-        for (int w = 0; w < active; w++) mx = fmaxf(mx, __ldcg(stat + (w * ROWS + r) * 2));
-        float sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        const float4 *v = reinterpret_cast<const float4 *>(part + (int64_t)r * D + d);
+#pragma unroll 8
         for (int w = 0; w < active; w++) {
-            const float2 ms = __ldcg(reinterpret_cast<const float2 *>(stat + (w * ROWS + r) * 2));
-            const float4 v = __ldcg(reinterpret_cast<const float4 *>(part + ((int64_t)w * ROWS + r) * D + d));
-            const float k = ms.x == -INFINITY ? 0.f : ex2(ms.x - mx);
-            sum += k * ms.y;
-            acc[0] += k * v.x, acc[1] += k * v.y, acc[2] += k * v.z, acc[3] += k * v.w;
+            const float4 x = __ldcg(v + (int64_t)w * (ROWS * D / 4));
+            const float k = wt[w * ROWS + r];
+            acc[0] += k * x.x, acc[1] += k * x.y, acc[2] += k * x.z, acc[3] += k * x.w;
         }
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-        for (int z = 0; z < 4; z++) acc[z] *= inv;
         store_act<T, 4>(static_cast<T *>(p.out) + (int64_t)(s.first + (r0 + r) / p.g) * p.ot +
                             (int64_t)(kvh * p.g + (r0 + r) % p.g) * D + d,
                         acc, p.vec);
     }
 }
 
-template <typename T, int D>
+template <typename T, int D, int ROWS>
 static const void *decode_fn(bool e4m3) {
-    return e4m3 ? (const void *)kv8_decode_kernel<T, D, true> : (const void *)kv8_decode_kernel<T, D, false>;
+    return e4m3 ? (const void *)kv8_decode_kernel<T, D, true, ROWS> : (const void *)kv8_decode_kernel<T, D, false, ROWS>;
 }
 template <typename T>
-static const void *decode_fn(int D, bool e4m3) {
-    return D == 64 ? decode_fn<T, 64>(e4m3) : decode_fn<T, 128>(e4m3);
+static const void *decode_fn(int D, bool e4m3, int rows) {
+    if constexpr (sizeof(T) == 2)
+        if (rows == 16) return D == 64 ? decode_fn<T, 64, 16>(e4m3) : decode_fn<T, 128, 16>(e4m3);
+    return D == 64 ? decode_fn<T, 64, 8>(e4m3) : decode_fn<T, 128, 8>(e4m3);
 }
 
 static Kv8Plan decode_plan(const vkq_kv8_cache &c, const vkq_kv8_batch &b, int dtype, int64_t heads, int causal,
                               int64_t window, int sms) {
     Kv8Plan q{};
-    q.rows = dtype == VKQ_F32 ? 8 : 16;
     const int64_t g = heads / c.kv_heads;
+    q.rows = dtype == VKQ_F32 || b.max_tokens * g <= 8 ? 8 : 16;
     q.row_tiles = (int)((b.max_tokens * g + q.rows - 1) / q.rows);
     q.tiles = b.batch * c.kv_heads * q.row_tiles;
     // keys that a tile can see: all, or a window and the tile's own tokens
@@ -475,12 +500,14 @@ static Kv8Plan decode_plan(const vkq_kv8_cache &c, const vkq_kv8_batch &b, int d
         if (w < keys) keys = w;
     }
     if (keys < 1) keys = 1;
-    // Ranges: enough CTAs for two on every SM with some to spare for ragged
-    // lengths, of at least one step a warp; none where the tiles alone suffice
-    // or are more than the workspace's head has counters for.
-    const int64_t want = 6 * (int64_t)sms;
-    int64_t splits = (want + q.tiles - 1) / q.tiles;
-    const int64_t most = (keys + kDecWarps * kDecStep - 1) / (kDecWarps * kDecStep);
+    // Ranges: one sequence fills the card once (its ranges are alike, and are
+    // joined by one CTA); several, of lengths that the host does not know, get
+    // three times as many, so that the long ones spread.  At least one step a
+    // warp (several sequences: four), and none where the tiles are more than
+    // the workspace's head has counters for.
+    const int64_t slots = dec_ctas(q.rows) * (int64_t)sms, least = kDecWarps * kDecStep * (b.batch > 1 ? 4 : 1);
+    int64_t splits = b.batch > 1 ? (3 * slots + q.tiles - 1) / q.tiles : slots / q.tiles;
+    const int64_t most = (keys + least - 1) / least;
     if (splits > most) splits = most;
     if (splits > 128) splits = 128;
     if (q.tiles > kHeadCounters || splits < 1) splits = 1;
@@ -523,6 +550,7 @@ cudaError_t kv8_attention(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_b
     p.q = a.q, p.out = a.out, p.qt = a.q_token, p.ot = a.out_token;
     p.heads = (int)a.heads, p.g = (int)(a.heads / c.kv_heads);
     p.row_tiles = q.row_tiles, p.splits = q.splits, p.chunk = q.chunk;
+    p.magic = kv8_magic((uint32_t)(c.page_size / kKv8Block));
     p.f = a.scale * 1.4426950408889634f;
     p.causal = a.causal, p.window = a.causal ? (int)a.window : 0;
     const int size = act_bytes(a.dtype);
@@ -530,9 +558,9 @@ cudaError_t kv8_attention(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_b
     p.count = static_cast<unsigned *>(a.workspace);
     p.part = reinterpret_cast<float *>(static_cast<char *>(a.workspace) + kWorkspaceCounterHead);
     p.stat = p.part + q.part_floats;
-    const void *fn = a.dtype == VKQ_F32   ? decode_fn<float>(c.head_dim, p.pool.e4m3)
-                     : a.dtype == VKQ_F16 ? decode_fn<__half>(c.head_dim, p.pool.e4m3)
-                                          : decode_fn<__nv_bfloat16>(c.head_dim, p.pool.e4m3);
+    const void *fn = a.dtype == VKQ_F32   ? decode_fn<float>(c.head_dim, p.pool.e4m3, q.rows)
+                     : a.dtype == VKQ_F16 ? decode_fn<__half>(c.head_dim, p.pool.e4m3, q.rows)
+                                          : decode_fn<__nv_bfloat16>(c.head_dim, p.pool.e4m3, q.rows);
     const size_t slots = (size_t)kDecWarps * kDecStages * (4 * kKv8Block * c.head_dim + 16);
     const size_t join = (size_t)kDecWarps * q.rows * (c.head_dim + 2) * sizeof(float);
     const size_t smem = slots > join ? slots : join;

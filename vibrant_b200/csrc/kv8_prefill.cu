@@ -194,25 +194,15 @@ __device__ __forceinline__ bool poll(uint32_t bar, uint32_t parity) {
     return false;
 }
 
-// 16 codes as 16 float16 (the conversions of kv8_attention.cu).
+// 16 codes as 16 float16.
 template <bool E4M3>
 __device__ __forceinline__ void codes_to_half(const uint4 &raw, uint32_t (&h)[8]) {
     const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        if constexpr (E4M3) {
-            const uint32_t a = prmt(w[i], 0u, 0x1404u), b = prmt(w[i], 0u, 0x3424u);
-            h[2 * i] = (a & 0x80008000u) | ((a >> 1) & 0x3F803F80u);
-            h[2 * i + 1] = (b & 0x80008000u) | ((b >> 1) & 0x3F803F80u);
-        } else {
-            const uint32_t u = w[i] ^ 0x80808080u;
-            const uint32_t a = prmt(u, 0x64646464u, 0x4140u), b = prmt(u, 0x64646464u, 0x4342u);
-            const __half2 off = __half2half2(__ushort_as_half(0x6480));
-            const __half2 x = __hsub2(*reinterpret_cast<const __half2 *>(&a), off);
-            const __half2 y = __hsub2(*reinterpret_cast<const __half2 *>(&b), off);
-            h[2 * i] = *reinterpret_cast<const uint32_t *>(&x);
-            h[2 * i + 1] = *reinterpret_cast<const uint32_t *>(&y);
-        }
+        const uint32_t u = kv8_unsign<E4M3>(w[i]);
+        h[2 * i] = kv8_widen<E4M3, false>(u);
+        h[2 * i + 1] = kv8_widen<E4M3, true>(u);
     }
 }
 
@@ -229,7 +219,6 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
     constexpr uint32_t TILE = 128 * D * 2;          // bytes of a float16 tile of 128 rows
     constexpr uint32_t HALF = kPreKeys * 128;       // its second half of 64 values
     constexpr float kUp = SPLIT ? 14.f : 6.f;       // e is held as 2^kUp e (at most 2^14)
-    constexpr float kOut = E4M3 ? 256.f : 1.f;      // e4m3 operands are 2^8 too small
     // TMEM columns: the scores (and, over them, e) of half or parity 0 and 1, the outputs
     constexpr uint32_t kS = 0, kO = 256;
     extern __shared__ __align__(1024) uint8_t smem[];  // two q tiles, the rings
@@ -317,7 +306,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
         for (int o = 1; o < RT; o <<= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
         const int e = min(max((int)(__float_as_uint(a) >> 23) - 127, -60), 127);
         const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
-        if (tid % RT == 0) row_f[lr] = p.f * __uint_as_float((uint32_t)(e - 14 + 127) << 23) * kOut;
+        if (tid % RT == 0) row_f[lr] = p.f * __uint_as_float((uint32_t)(e - 14 + 127) << 23);
         const uint32_t dst = q_tile + (SPLIT ? 0u : (uint32_t)(lr / 128) * TILE);
 #pragma unroll
         for (int c = 0; c < PV; c += 8) {
@@ -406,14 +395,14 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PreRegs<SPLIT>::issue));
         if (warp == 13 && n > 0) {
             // the tiles' pages: lane b takes block b
-            const uint32_t per_page = (uint32_t)(p.pool.page / kKv8Block);
+            const uint32_t per_page = (uint32_t)(p.pool.page / kKv8Block), magic = 0xffffffffu / per_page + 1u;
             // The block of the layer's pool ([page][kv head][block]): 0 past the range
             // and, with bad_flag, for a page out of range.  (Below 2^31: a pool of
             // that many blocks would be 2 TB.)
             auto look = [&](int j) -> uint32_t {
                 const int key = k_lo + j * kPreKeys + lane * kKv8Block;
                 if (lane >= kPreBlocks || j >= n || key >= k_hi) return 0;
-                const uint32_t blk = (uint32_t)key / kKv8Block, lp = blk / per_page;
+                const uint32_t blk = (uint32_t)key / kKv8Block, lp = kv8_div(blk, per_page, magic);
                 const int id = kv8_page(p.pool, s, (int)lp);
                 if (id < 0) bad_flag = 1;
                 return id < 0 ? 0u : ((uint32_t)id * (uint32_t)p.pool.kv_heads + (uint32_t)kvh) * per_page + (blk - lp * per_page);
@@ -577,7 +566,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
                 d[0] = make_float4(v[0], v[1], v[2], v[3]);
                 d[1] = make_float4(v[4], v[5], v[6], v[7]);
             } else {
-                const float inv = l == 0.f ? 0.f : kOut / l;
+                const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
                 for (int u = 0; u < 8; u++) v[u] *= inv;
                 store_act<T, 8>(out_row + c, v, p.vec);
@@ -794,7 +783,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
             sum += k * ms.y;
             acc[0] += k * v.x, acc[1] += k * v.y, acc[2] += k * v.z, acc[3] += k * v.w;
         }
-        const float inv = sum == 0.f ? 0.f : kOut / sum;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
         for (int z = 0; z < 4; z++) acc[z] *= inv;
         store_act<T, 4>(static_cast<T *>(p.out) + (int64_t)(s.first + (r0 + r) / p.g) * p.ot +
