@@ -232,7 +232,7 @@ int vkq_kv8_append(int device, const vkq_kv8_cache *cache, int64_t layer, const 
         }
     }
     if (batch->tokens == 0) return VKQ_OK;
-    if (kv8_append_warps(*cache, *batch, heads, q != nullptr) > int64_t(1) << 32) {
+    if (kv8_append_ctas(*cache, *batch, q != nullptr) > INT32_MAX) {
         set_error("%s: batch of %lld sequences of up to %lld tokens is too large for one call", who,
                   (long long)batch->batch, (long long)batch->max_tokens);
         return VKQ_ERR_UNSUPPORTED;
@@ -258,7 +258,7 @@ int vkq_kv8_read(int device, const vkq_kv8_cache *cache, int64_t layer, const vk
         set_error("%s: the lists must be 4-byte and the outputs 16-byte aligned", who);
         return VKQ_ERR_MISALIGNED;
     }
-    return check_launch(kv8_read(*cache, layer, *batch, seq, pos, n, dtype, k_out, v_out, (cudaStream_t)stream, device),
+    return check_launch(kv8_read(*cache, layer, *batch, seq, pos, n, dtype, k_out, v_out, (cudaStream_t)stream),
                         "KV cache read");
 }
 

@@ -12,18 +12,19 @@
 // last scale (with free scales, 15 appends could add 15 half steps).  The cost
 // is up to one bit of the int8 code's range; e4m3 loses nothing.
 //
-// One warp takes one block of K or V: the 16 rows sit in its registers
-// (D / 32 values of each row a lane), the maximum is one butterfly, and no
-// other warp touches the block, so there are no atomics and the result does
-// not depend on the order of anything.  Bytes bound a prompt, latency a decode
-// step; q's rotation rides in the same launch (warps past the blocks'), which
-// saves a launch a layer.
+// One CTA takes one block of K or V: four rows a warp (D / 32 values of a row a
+// lane), the maximum over the warps through shared memory.  No other CTA
+// touches the block, so there are no atomics and the result does not depend on
+// the order of anything.  Bytes bound a prompt, latency a decode step; q's
+// rotation rides in the same launch (CTAs past the blocks', a few tokens each),
+// which saves a launch a layer.
 #include <cstdint>
 
 #include "../../include/vkq.h"
 #include "act.cuh"
 #include "kq_device.cuh"
 #include "kv8.cuh"
+#include "rotary.cuh"
 #include "vkq_internal.h"
 
 namespace vkq {
@@ -35,6 +36,8 @@ __device__ __forceinline__ void kv8_bad() { atomicExch(&g_kv8_status, VKQ_ERR_IN
 constexpr int kAppThreads = 128;
 constexpr int kAppWarps = kAppThreads / 32;
 
+constexpr int kAppRows = kKv8Block / kAppWarps;  // rows of a block that a warp takes
+
 struct AppendParams {
     Kv8Pool pool;
     Kv8Batch batch;
@@ -44,120 +47,170 @@ struct AppendParams {
     const float *cos_t, *sin_t;
     int64_t max_seq;
     int heads, rot;
-    int max_blocks;       // blocks that one sequence's new tokens can touch
-    int64_t block_items;  // warps of blocks: batch * max_blocks * kv_heads * 2
-    int64_t items;        // and of q: tokens * ceil(heads / kAppHeads)
-    bool half, vec_kv, vec_q;
+    uint32_t max_blocks;   // blocks that one sequence's new tokens can touch
+    uint32_t block_ctas;   // batch * max_blocks * kv_heads * 2
+    int q_tokens, q_items; // tokens of a CTA of q's, items of a token
+    bool half, vec_kv, vec_t, vec_q;  // a lane's values as one vector: k and v, the tables; q by 16-byte pieces
 };
-constexpr int kAppHeads = 4;  // heads of q that a warp rotates
+constexpr int kAppMaxTokens = 8;
 
-// The lane's N = D / 32 values of one row, rotated at position ps (table row):
-// interleaved pairs lie in the lane; a half pair's partner is loaded as well.
-// Any rot: values past it are as they are.
-template <typename T, int D>
-__device__ __forceinline__ void load_turned(const T *row, float (&x)[D / 32], int lane, bool vec, bool rotate,
-                                            const float *cos_t, const float *sin_t, int64_t ps, int rot, bool half) {
-    constexpr int N = D / 32;
-    const int d0 = lane * N, h = rot / 2;
-    load_act<T, N>(row + d0, x, vec);
-    if (!rotate) return;
-    const float *ct = cos_t + ps * h, *st = sin_t + ps * h;
-    if (!half) {
+// How a lane's N = D / 32 values of a head turn: interleaved pairs lie in the
+// lane, a half pair's partners in another lane's row part (loaded as well).
+// `vec`: the lane's values have one role, so partners and table entries are
+// vectors; else each value is looked at by itself.
+struct LaneTurn {
+    int d0, h, rot;    // the lane's first dimension; rot / 2; rot
+    bool rotate, half, vec;
+};
+template <int N>
+__device__ __forceinline__ LaneTurn lane_turn(const AppendParams &p, int lane, bool rotate) {
+    return LaneTurn{lane * N, p.rot / 2, p.rot, rotate, p.half, p.rot % (2 * N) == 0 && p.vec_t};
+}
+// The table entries of the lane's values at position ps (vec only).
+template <int N>
+__device__ __forceinline__ void load_entries(const AppendParams &p, const LaneTurn &l, int64_t ps, float (&c)[N],
+                                             float (&s)[N]) {
+    if (!l.rotate || !l.vec || l.d0 >= l.rot) return;
+    const int64_t row = ps * l.h;
+    if (l.half) {
+        const int64_t e = row + (l.d0 < l.h ? l.d0 : l.d0 - l.h);
+        load_act<float, N>(p.cos_t + e, c, true);
+        load_act<float, N>(p.sin_t + e, s, true);
+    } else {
+        float a[N / 2], b[N / 2];
+        if constexpr (N == 4) {
+            const float2 x = *reinterpret_cast<const float2 *>(p.cos_t + row + l.d0 / 2);
+            const float2 y = *reinterpret_cast<const float2 *>(p.sin_t + row + l.d0 / 2);
+            a[0] = x.x, a[1] = x.y, b[0] = y.x, b[1] = y.y;
+        } else {
+            a[0] = p.cos_t[row + l.d0 / 2], b[0] = p.sin_t[row + l.d0 / 2];
+        }
 #pragma unroll
-        for (int i = 0; i < N; i += 2)
-            if (d0 + i < rot) turn(x[i], x[i + 1], ct[(d0 + i) / 2], st[(d0 + i) / 2]);
+        for (int i = 0; i < N / 2; i++) c[i] = a[i], s[i] = b[i];
+    }
+}
+// The lane's values x of `row` and their partners y (half, vec).
+template <typename T, int N>
+__device__ __forceinline__ void load_pair(const T *row, const LaneTurn &l, bool vec, float (&x)[N], float (&y)[N]) {
+    load_act<T, N>(row + l.d0, x, vec);
+    if (l.rotate && l.vec && l.half && l.d0 < l.rot) load_act<T, N>(row + (l.d0 < l.h ? l.d0 + l.h : l.d0 - l.h), y, vec);
+}
+template <typename T, int N>
+__device__ __forceinline__ void turn_lane(const AppendParams &p, const T *row, const LaneTurn &l, int64_t ps,
+                                          const float (&c)[N], const float (&s)[N], float (&x)[N], float (&y)[N]) {
+    if (!l.rotate || l.d0 >= l.rot) return;
+    if (l.vec) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            if (l.half) {
+                float a = l.d0 < l.h ? x[i] : y[i], b = l.d0 < l.h ? y[i] : x[i];
+                turn(a, b, c[i], s[i]);
+                x[i] = l.d0 < l.h ? a : b;
+            } else if (i % 2 == 0) {
+                turn(x[i], x[i + 1], c[i / 2], s[i / 2]);
+            }
+        }
         return;
     }
-#pragma unroll
+    const float *ct = p.cos_t + ps * l.h, *st = p.sin_t + ps * l.h;
     for (int i = 0; i < N; i++) {
-        const int d = d0 + i;
-        if (d < h) {
-            float b = to_f32<T>(row[d + h]);
+        const int d = l.d0 + i;
+        if (d >= l.rot) break;
+        if (!l.half) {
+            if (i % 2 == 0) turn(x[i], x[i + 1], ct[d / 2], st[d / 2]);
+        } else if (d < l.h) {
+            float b = to_f32<T>(row[d + l.h]);
             turn(x[i], b, ct[d], st[d]);
-        } else if (d < rot) {
-            float a = to_f32<T>(row[d - h]);
-            turn(a, x[i], ct[d - h], st[d - h]);
+        } else {
+            float a = to_f32<T>(row[d - l.h]);
+            turn(a, x[i], ct[d - l.h], st[d - l.h]);
         }
     }
 }
 
 template <typename T, int D>
-__device__ void append_block(const AppendParams &p, int64_t item, int lane) {
+__device__ void append_block(const AppendParams &p, uint32_t cta) {
     constexpr int N = D / 32;
-    const bool is_v = item & 1;
-    int64_t r = item >> 1;
-    const int kvh = p.pool.kv_heads;
+    __shared__ float amax[kAppWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const bool is_v = cta & 1;
+    uint32_t r = cta >> 1;
+    const uint32_t kvh = (uint32_t)p.pool.kv_heads;
     const int h = (int)(r % kvh);
     r /= kvh;
     const int j = (int)(r % p.max_blocks);
-    const int64_t b = r / p.max_blocks;
-    const Kv8Seq s = kv8_seq(p.batch, p.pool.page, b);
+    const Kv8Seq s = kv8_seq(p.batch, p.pool.page, r / p.max_blocks);
     const bool rotate = p.cos_t != nullptr;
     if (!s.ok || s.n > s.len || (rotate && s.len > p.max_seq)) {
-        if (lane == 0 && j == 0) kv8_bad();
+        if (threadIdx.x == 0 && j == 0) kv8_bad();
         return;
     }
     const int start = s.len - s.n;
-    const int blk = start / kKv8Block + j;
-    const int pos0 = blk * kKv8Block;
+    const int pos0 = (start / kKv8Block + j) * kKv8Block;
     if (s.n == 0 || pos0 >= s.len) return;
     const int lo = max(start - pos0, 0), hi = min(s.len - pos0, kKv8Block);  // the block's new rows
+    const T *src = static_cast<const T *>(is_v ? p.v : p.k) + (int64_t)(s.first + pos0 - start) * (is_v ? p.vt : p.kt) +
+                   h * D;
+    const int64_t stride = is_v ? p.vt : p.kt;
+    const LaneTurn lt = lane_turn<N>(p, lane, rotate && !is_v);
+    float x[kAppRows][N], y[kAppRows][N], c[kAppRows][N], sn[kAppRows][N];
+#pragma unroll
+    for (int i = 0; i < kAppRows; i++) {
+        const int t = warp + i * kAppWarps;
+        if (t < lo || t >= hi) continue;
+        load_pair<T, N>(src + t * stride, lt, p.vec_kv, x[i], y[i]);
+        load_entries<N>(p, lt, pos0 + t, c[i], sn[i]);
+    }
     const int id = kv8_page(p.pool, s, pos0 / p.pool.page);
     if (id < 0) {
-        if (lane == 0) kv8_bad();
+        if (threadIdx.x == 0) kv8_bad();
         return;
     }
     const int in_page = pos0 % p.pool.page;
     const int64_t ph = (int64_t)id * kvh + h;
     float *scale = (is_v ? p.pool.vs : p.pool.ks) + ph * (p.pool.page / kKv8Block) + in_page / kKv8Block;
     uint8_t *codes = (is_v ? p.pool.v : p.pool.k) + (ph * p.pool.page + in_page) * D + lane * N;
-    const T *src = static_cast<const T *>(is_v ? p.v : p.k) + (int64_t)(s.first + pos0 - start) * (is_v ? p.vt : p.kt) +
-                   h * D;
-    const int64_t stride = is_v ? p.vt : p.kt;
     const float s_old = lo > 0 ? *scale : 0.f;
-    float x[kKv8Block][N];
     float a = 0.f;
 #pragma unroll
-    for (int t = 0; t < kKv8Block; t++) {
-        if (t >= lo && t < hi) {
-            load_turned<T, D>(src + t * stride, x[t], lane, p.vec_kv, rotate && !is_v, p.cos_t, p.sin_t, pos0 + t, p.rot,
-                              p.half);
+    for (int i = 0; i < kAppRows; i++) {
+        const int t = warp + i * kAppWarps;
+        if (t < lo || t >= hi) continue;
+        turn_lane<T, N>(p, src + t * stride, lt, pos0 + t, c[i], sn[i], x[i], y[i]);
 #pragma unroll
-            for (int i = 0; i < N; i++) {
-                const float m = fabsf(x[t][i]);
-                if (m <= 3.402823466e38f) a = fmaxf(a, m);  // finite
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; i++) x[t][i] = 0.f;
+        for (int u = 0; u < N; u++) {
+            const float m = fabsf(x[i][u]);
+            if (m <= 3.402823466e38f) a = fmaxf(a, m);  // finite
         }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+    if (lane == 0) amax[warp] = a;
+    __syncthreads();  // every thread has read the old scale, too
+#pragma unroll
+    for (int w = 0; w < kAppWarps; w++) a = fmaxf(a, amax[w]);
     const float sc = fmaxf(s_old, kv8_scale(a, p.pool.e4m3));
-    if (lo > 0 && sc > s_old) {
-        const float ratio = __fdiv_rn(s_old, sc);
-        for (int t = 0; t < lo; t++) {
-            uint8_t *c = codes + t * D;
-            uint32_t w = N == 4 ? *reinterpret_cast<uint32_t *>(c) : *reinterpret_cast<uint16_t *>(c), o = 0;
+    const bool grew = lo > 0 && sc > s_old;
+    const float inv = __fdiv_rn(1.f, sc), ratio = grew ? __fdiv_rn(s_old, sc) : 1.f;
 #pragma unroll
-            for (int i = 0; i < N; i++)
-                o |= kv8_encode(kv8_decode((w >> (8 * i)) & 0xFFu, p.pool.e4m3) * ratio, p.pool.e4m3) << (8 * i);
-            if (N == 4) *reinterpret_cast<uint32_t *>(c) = o;
-            else *reinterpret_cast<uint16_t *>(c) = (uint16_t)o;
-        }
-    }
-    const float inv = __fdiv_rn(1.f, sc);
-#pragma unroll
-    for (int t = 0; t < kKv8Block; t++) {
-        if (t < lo || t >= hi) continue;
+    for (int i = 0; i < kAppRows; i++) {
+        const int t = warp + i * kAppWarps;
+        if (t >= hi || (t < lo && !grew)) continue;
+        uint8_t *out = codes + t * D;
         uint32_t o = 0;
+        if (t < lo) {
+            const uint32_t w = N == 4 ? *reinterpret_cast<uint32_t *>(out) : *reinterpret_cast<uint16_t *>(out);
 #pragma unroll
-        for (int i = 0; i < N; i++) o |= kv8_encode(x[t][i] * inv, p.pool.e4m3) << (8 * i);
-        if (N == 4) *reinterpret_cast<uint32_t *>(codes + t * D) = o;
-        else *reinterpret_cast<uint16_t *>(codes + t * D) = (uint16_t)o;
+            for (int u = 0; u < N; u++)
+                o |= kv8_encode(kv8_decode((w >> (8 * u)) & 0xFFu, p.pool.e4m3) * ratio, p.pool.e4m3) << (8 * u);
+        } else {
+#pragma unroll
+            for (int u = 0; u < N; u++) o |= kv8_encode(x[i][u] * inv, p.pool.e4m3) << (8 * u);
+        }
+        if (N == 4) *reinterpret_cast<uint32_t *>(out) = o;
+        else *reinterpret_cast<uint16_t *>(out) = (uint16_t)o;
     }
-    if (lane == 0) *scale = sc;
+    if (threadIdx.x == 0) *scale = sc;
 }
 
 // The sequence of token t: the last b with cu[b] <= t (empty sequences skipped).
@@ -172,38 +225,48 @@ __device__ __forceinline__ int64_t seq_of_token(const Kv8Batch &b, int64_t t) {
     return lo;
 }
 
+// q_tokens tokens of q: their positions first, then the items of all of them.
 template <typename T, int D>
-__device__ void append_q(const AppendParams &p, int64_t item, int lane) {
-    constexpr int N = D / 32;
-    const int groups = (p.heads + kAppHeads - 1) / kAppHeads;
-    const int64_t t = item / groups;
-    const int h0 = (int)(item - t * groups) * kAppHeads;
-    const int64_t b = seq_of_token(p.batch, t);
-    if (b >= p.batch.batch) return;
-    const Kv8Seq s = kv8_seq(p.batch, p.pool.page, b);
-    if (!s.ok || s.n > s.len || s.len > p.max_seq || t < s.first || t >= s.first + s.n) return;
-    const int64_t ps = s.len - s.n + (t - s.first);
-    const T *q = static_cast<const T *>(p.q) + t * p.qt;
-    T *o = static_cast<T *>(p.q_out) + t * p.qot;
-    float x[kAppHeads][N];
-#pragma unroll
-    for (int u = 0; u < kAppHeads; u++)
-        if (h0 + u < p.heads)
-            load_turned<T, D>(q + (h0 + u) * D, x[u], lane, p.vec_q, true, p.cos_t, p.sin_t, ps, p.rot, p.half);
-    __syncwarp();  // q_out may be q: a lane has read its partner before any lane writes
-#pragma unroll
-    for (int u = 0; u < kAppHeads; u++)
-        if (h0 + u < p.heads) store_act<T, N>(o + (h0 + u) * D + lane * N, x[u], p.vec_q);
+__device__ void append_q(const AppendParams &p, uint32_t cta) {
+    __shared__ int pos[kAppMaxTokens];
+    const int64_t t0 = (int64_t)cta * p.q_tokens;
+    if ((int)threadIdx.x < p.q_tokens) {
+        const int64_t t = t0 + threadIdx.x, b = t < p.batch.tokens ? seq_of_token(p.batch, t) : p.batch.batch;
+        int at = -1;
+        if (b < p.batch.batch) {
+            const Kv8Seq s = kv8_seq(p.batch, p.pool.page, b);
+            if (s.ok && s.n <= s.len && s.len <= p.max_seq && t >= s.first && t < s.first + s.n)
+                at = s.len - s.n + (int)(t - s.first);
+        }
+        pos[threadIdx.x] = at;
+    }
+    __syncthreads();
+    const int groups = (p.heads + kRotHeads - 1) / kRotHeads;
+    for (int x = threadIdx.x; x < p.q_tokens * p.q_items; x += kAppThreads) {
+        const int i = x / p.q_items, rest = x - i * p.q_items;
+        if (pos[i] < 0) continue;
+        const T *q = static_cast<const T *>(p.q) + (t0 + i) * p.qt;
+        T *o = static_cast<T *>(p.q_out) + (t0 + i) * p.qot;
+        if (p.vec_q) {
+            const int pieces = p.q_items / groups, g = rest / pieces, j = rest - g * pieces, h0 = g * kRotHeads;
+            auto row = [&]() -> int64_t { return pos[i]; };
+            if (p.half)
+                rotary_item<T, true>(q + h0 * D, D, o + h0 * D, D, p.heads - h0, j, D, p.rot, p.cos_t, p.sin_t, false, row);
+            else
+                rotary_item<T, false>(q + h0 * D, D, o + h0 * D, D, p.heads - h0, j, D, p.rot, p.cos_t, p.sin_t, false, row);
+        } else {
+            const int per = D - p.rot / 2, h = rest / per;
+            rotary_one<T>(q + h * D, o + h * D, rest - h * per, p.rot, p.half, p.cos_t, p.sin_t, false, pos[i]);
+        }
+    }
 }
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kAppThreads) append_kernel(const AppendParams p) {
     pdl_wait();
     pdl_launch_dependents();
-    const int lane = threadIdx.x & 31;
-    const int64_t item = (int64_t)blockIdx.x * kAppWarps + (threadIdx.x >> 5);
-    if (item < p.block_items) append_block<T, D>(p, item, lane);
-    else if (item < p.items) append_q<T, D>(p, item - p.block_items, lane);
+    if (blockIdx.x < p.block_ctas) append_block<T, D>(p, blockIdx.x);
+    else append_q<T, D>(p, blockIdx.x - p.block_ctas);
 }
 
 // ---- reading rows back ------------------------------------------------------
@@ -211,47 +274,72 @@ struct ReadParams {
     Kv8Pool pool;
     Kv8Batch batch;
     const int *seq, *pos;
-    int64_t items;  // n * kv_heads * D / 4
+    int64_t n;
+    int rows;  // of a CTA
     void *k_out, *v_out;
 };
+constexpr int kReadThreads = 256, kReadRows = 8;
 
-// Four values a thread: bytes bound it, and consecutive threads write 16 (8)
-// consecutive bytes each.
-template <typename T>
-__global__ void __launch_bounds__(256) read_kernel(const ReadParams p) {
+// A CTA takes eight rows (one, where there are few): one thread a row finds its page, then every thread
+// reads the same four values of each row.  Bytes bound it; consecutive threads
+// write 16 (8) consecutive bytes each.
+template <typename T, bool E4M3>
+__global__ void __launch_bounds__(kReadThreads) read_kernel(const ReadParams p) {
+    __shared__ int64_t row_at[kReadRows], scale_at[kReadRows];  // of KV head 0
     pdl_wait();
     pdl_launch_dependents();
-    const int quads = p.pool.D / 4, kvh = p.pool.kv_heads;
-    for (int64_t it = (int64_t)blockIdx.x * 256 + threadIdx.x; it < p.items; it += (int64_t)gridDim.x * 256) {
-        const int64_t row = it / ((int64_t)quads * kvh);
-        const int rest = (int)(it - row * quads * kvh);
-        const int h = rest / quads, d = (rest - h * quads) * 4;
-        const int64_t b = p.seq[row];
-        const int ps = p.pos[row];
-        int id = -1;
-        if (b >= 0 && b < p.batch.batch) {
-            const Kv8Seq s = kv8_seq(p.batch, p.pool.page, b);
-            if (s.ok && ps >= 0 && ps < s.len) id = kv8_page(p.pool, s, ps / p.pool.page);
-        }
-        float kx[4], vx[4];
-        if (id < 0) {
-            if (rest == 0) kv8_bad();
-            kx[0] = kx[1] = kx[2] = kx[3] = vx[0] = vx[1] = vx[2] = vx[3] = __int_as_float(0x7fc00000);
-        } else {
-            const int at = ps % p.pool.page;
-            const int64_t ph = (int64_t)id * kvh + h;
-            const int64_t e = (ph * p.pool.page + at) * p.pool.D + d, se = ph * (p.pool.page / kKv8Block) + at / kKv8Block;
-            const uint32_t kw = *reinterpret_cast<const uint32_t *>(p.pool.k + e);
-            const uint32_t vw = *reinterpret_cast<const uint32_t *>(p.pool.v + e);
-            const float ks = p.pool.ks[se], vs = p.pool.vs[se];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                kx[i] = kv8_decode((kw >> (8 * i)) & 0xFFu, p.pool.e4m3) * ks;
-                vx[i] = kv8_decode((vw >> (8 * i)) & 0xFFu, p.pool.e4m3) * vs;
+    const int64_t r0 = (int64_t)blockIdx.x * p.rows;
+    const int D = p.pool.D, page = p.pool.page;
+    if ((int)threadIdx.x < p.rows) {
+        int64_t at = -1, sc = 0;
+        const int64_t r = r0 + threadIdx.x;
+        if (r < p.n) {
+            const int64_t b = p.seq[r];
+            const int ps = p.pos[r];
+            if (b >= 0 && b < p.batch.batch) {
+                const Kv8Seq s = kv8_seq(p.batch, page, b);
+                if (s.ok && ps >= 0 && ps < s.len) {
+                    const int id = kv8_page(p.pool, s, ps / page), in = ps % page;
+                    if (id >= 0) {
+                        at = ((int64_t)id * p.pool.kv_heads * page + in) * D;
+                        sc = (int64_t)id * p.pool.kv_heads * (page / kKv8Block) + in / kKv8Block;
+                    }
+                }
             }
+            if (at < 0) kv8_bad();
         }
-        if (p.k_out) store_act<T, 4>(static_cast<T *>(p.k_out) + it * 4, kx, true);
-        if (p.v_out) store_act<T, 4>(static_cast<T *>(p.v_out) + it * 4, vx, true);
+        row_at[threadIdx.x] = at;
+        scale_at[threadIdx.x] = sc;
+    }
+    __syncthreads();
+    const int quads = D / 4, width = p.pool.kv_heads * quads, rows = (int)min((int64_t)p.rows, p.n - r0);
+    for (int x = threadIdx.x; x < width; x += kReadThreads) {
+        const int h = x / quads, d = (x - h * quads) * 4;
+#pragma unroll
+        for (int i = 0; i < kReadRows; i++) {
+            if (i >= rows) break;
+            float kx[4], vx[4];
+            if (row_at[i] < 0) {
+                kx[0] = kx[1] = kx[2] = kx[3] = vx[0] = vx[1] = vx[2] = vx[3] = __int_as_float(0x7fc00000);
+            } else {
+                const int64_t e = row_at[i] + (int64_t)h * page * D + d, se = scale_at[i] + h * (page / kKv8Block);
+                const uint32_t kw = kv8_unsign<E4M3>(*reinterpret_cast<const uint32_t *>(p.pool.k + e));
+                const uint32_t vw = kv8_unsign<E4M3>(*reinterpret_cast<const uint32_t *>(p.pool.v + e));
+                const float ks = p.pool.ks[se], vs = p.pool.vs[se];
+                const uint32_t w[4] = {kv8_widen<E4M3, false>(kw), kv8_widen<E4M3, true>(kw), kv8_widen<E4M3, false>(vw),
+                                       kv8_widen<E4M3, true>(vw)};
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&w[u]));
+                    const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&w[2 + u]));
+                    kx[2 * u] = a.x * ks, kx[2 * u + 1] = a.y * ks;
+                    vx[2 * u] = b.x * vs, vx[2 * u + 1] = b.y * vs;
+                }
+            }
+            const int64_t o = (r0 + i) * width * 4 + x * 4;
+            if (p.k_out) store_act<T, 4>(static_cast<T *>(p.k_out) + o, kx, true);
+            if (p.v_out) store_act<T, 4>(static_cast<T *>(p.v_out) + o, vx, true);
+        }
     }
 }
 
@@ -274,9 +362,11 @@ static const void *append_fn(int D) {
     return D == 64 ? (const void *)append_kernel<T, 64> : (const void *)append_kernel<T, 128>;
 }
 
-int64_t kv8_append_warps(const vkq_kv8_cache &c, const vkq_kv8_batch &b, int64_t heads, bool q) {
-    const int64_t max_blocks = (b.max_tokens + kKv8Block - 2) / kKv8Block + 1;
-    return b.batch * max_blocks * c.kv_heads * 2 + (q ? b.tokens * ((heads + kAppHeads - 1) / kAppHeads) : 0);
+static int64_t append_blocks(const vkq_kv8_cache &c, const vkq_kv8_batch &b) {
+    return b.batch * ((b.max_tokens + kKv8Block - 2) / kKv8Block + 1) * c.kv_heads * 2;
+}
+int64_t kv8_append_ctas(const vkq_kv8_cache &c, const vkq_kv8_batch &b, bool q) {
+    return append_blocks(c, b) + (q ? b.tokens : 0);
 }
 
 cudaError_t kv8_append(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_batch &b, const Kv8AppendArgs &a,
@@ -288,35 +378,47 @@ cudaError_t kv8_append(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_batc
     p.kt = a.k_token, p.vt = a.v_token, p.qt = a.q_token, p.qot = a.q_out_token;
     p.cos_t = a.cos_t, p.sin_t = a.sin_t, p.max_seq = a.max_seq;
     p.heads = (int)a.heads, p.rot = (int)a.rot_dim, p.half = a.layout == VKQ_ROPE_HALF;
-    p.max_blocks = (int)((b.max_tokens + kKv8Block - 2) / kKv8Block + 1);
-    p.block_items = b.batch * p.max_blocks * c.kv_heads * 2;
-    p.items = kv8_append_warps(c, b, a.heads, a.q != nullptr);
+    p.max_blocks = (uint32_t)((b.max_tokens + kKv8Block - 2) / kKv8Block + 1);
+    p.block_ctas = (uint32_t)append_blocks(c, b);
     // a lane's D / 32 values as one vector
     const int size = act_bytes(a.dtype);
     const uintptr_t lane = (uintptr_t)(c.head_dim / 32 * size) - 1;
     p.vec_kv = (((uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)(a.k_token * size) | (uintptr_t)(a.v_token * size)) & lane) == 0;
-    p.vec_q = (((uintptr_t)a.q | (uintptr_t)a.q_out | (uintptr_t)(a.q_token * size) | (uintptr_t)(a.q_out_token * size)) &
-               lane) == 0;
+    p.vec_t = (((uintptr_t)a.cos_t | (uintptr_t)a.sin_t) & 15u) == 0 && a.rot_dim % 8 == 0;
+    int64_t ctas = p.block_ctas;
+    if (a.q) {
+        const uintptr_t bits = (uintptr_t)a.q | (uintptr_t)a.q_out | (uintptr_t)a.cos_t | (uintptr_t)a.sin_t |
+                               (uintptr_t)(a.q_token * size) | (uintptr_t)(a.q_out_token * size);
+        p.vec_q = rotary_vec(bits, a.rot_dim);
+        const int pieces = size == 4 ? rotary_pieces<float>(c.head_dim, p.rot, p.half)
+                                     : rotary_pieces<__half>(c.head_dim, p.rot, p.half);
+        p.q_items = p.vec_q ? (p.heads + kRotHeads - 1) / kRotHeads * pieces : p.heads * (c.head_dim - p.rot / 2);
+        // many tokens share the search for their sequence; few are spread
+        p.q_tokens = b.tokens >= 1024 ? kAppMaxTokens : 1;
+        ctas += (b.tokens + p.q_tokens - 1) / p.q_tokens;
+    }
     const void *fn = a.dtype == VKQ_F32   ? append_fn<float>(c.head_dim)
                      : a.dtype == VKQ_F16 ? append_fn<__half>(c.head_dim)
                                           : append_fn<__nv_bfloat16>(c.head_dim);
-    return launch(fn, (p.items + kAppWarps - 1) / kAppWarps, kAppThreads, &p, s);
+    return launch(fn, ctas, kAppThreads, &p, s);
+}
+
+template <typename T>
+static const void *read_fn(bool e4m3) {
+    return e4m3 ? (const void *)read_kernel<T, true> : (const void *)read_kernel<T, false>;
 }
 
 cudaError_t kv8_read(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_batch &b, const int *seq, const int *pos,
-                     int64_t n, int dtype, void *k_out, void *v_out, cudaStream_t s, int device) {
+                     int64_t n, int dtype, void *k_out, void *v_out, cudaStream_t s) {
     ReadParams p{};
     p.pool = kv8_pool(c, layer);
     p.batch = kv8_batch(b);
-    p.seq = seq, p.pos = pos, p.k_out = k_out, p.v_out = v_out;
-    p.items = n * c.kv_heads * (c.head_dim / 4);
-    int64_t blocks = (p.items + 255) / 256;
-    const int64_t cap = 64 * (int64_t)device_sm_count(device);
-    if (blocks > cap) blocks = cap;
-    const void *fn = dtype == VKQ_F32   ? (const void *)read_kernel<float>
-                     : dtype == VKQ_F16 ? (const void *)read_kernel<__half>
-                                        : (const void *)read_kernel<__nv_bfloat16>;
-    return launch(fn, blocks, 256, &p, s);
+    p.seq = seq, p.pos = pos, p.n = n, p.k_out = k_out, p.v_out = v_out;
+    p.rows = n >= 8192 ? kReadRows : 1;
+    const void *fn = dtype == VKQ_F32   ? read_fn<float>(p.pool.e4m3)
+                     : dtype == VKQ_F16 ? read_fn<__half>(p.pool.e4m3)
+                                        : read_fn<__nv_bfloat16>(p.pool.e4m3);
+    return launch(fn, (n + p.rows - 1) / p.rows, kReadThreads, &p, s);
 }
 
 int kv8_read_status() {

@@ -15,6 +15,7 @@
 #include "../../include/vkq.h"
 #include "act.cuh"
 #include "kq_device.cuh"
+#include "rotary.cuh"
 #include "vkq_internal.h"
 
 namespace vkq {
@@ -22,7 +23,6 @@ namespace vkq {
 static __device__ int g_rotary_status;
 
 constexpr int kRotThreads = 128;
-constexpr int kRotHeads = 4;
 
 struct RotaryParams {
     const void *x;
@@ -35,80 +35,31 @@ struct RotaryParams {
     bool half, inverse;
 };
 
-// N pairs' table entries; aligned because N divides rot / 2 or the row is read one by one.
-template <int N>
-__device__ __forceinline__ void load_table(const float *t, float (&r)[N], bool vec) {
-    load_act<float, N>(t, r, vec);
-}
-
-// The vector path: heads in 16-byte pieces of V elements, rot a multiple of
-// 2V, aligned rows.  Interleaved: piece j of D / V (the rotated ones first);
-// half: the rot / 2V partner pairs, then the pieces past rot.
-template <typename T, bool HALF>
+template <typename T, bool HALF, typename I>
 __global__ void __launch_bounds__(kRotThreads) rotary_vec_kernel(const RotaryParams p) {
-    constexpr int V = 16 / (int)sizeof(T);
-    constexpr int NP = HALF ? V : V / 2;  // pairs of an item
     pdl_wait();
     pdl_launch_dependents();
-    const int64_t stride = (int64_t)gridDim.x * kRotThreads;
-    for (int64_t it = (int64_t)blockIdx.x * kRotThreads + threadIdx.x; it < p.items; it += stride) {
-        const int64_t tg = it / p.pieces;
-        const int j = (int)(it - tg * p.pieces);
-        const int64_t t = tg / p.groups;
-        const int h0 = (int)(tg - t * p.groups) * kRotHeads;
+    const I items = (I)p.items, stride = (I)gridDim.x * kRotThreads;
+    for (I it = (I)blockIdx.x * kRotThreads + threadIdx.x; it < items; it += stride) {
+        const I tg = it / (I)p.pieces;
+        const int j = (int)(it - tg * (I)p.pieces);
+        const I t = tg / (I)p.groups;
+        const int h0 = (int)(tg - t * (I)p.groups) * kRotHeads;
         const int ps = p.pos[t];
-        if (ps < 0 || ps >= p.max_seq) {
-            atomicExch(&g_rotary_status, VKQ_ERR_INVALID_ARGUMENT);
-            continue;
-        }
-        const int turned = HALF ? p.rot / (2 * V) : p.rot / V;
-        const bool turns = j < turned;
-        // first element of the piece, and of its partner
-        const int a0 = HALF && !turns ? p.rot + (j - turned) * V : j * V;
-        const int b0 = HALF ? a0 + p.rot / 2 : a0;
-        float c[NP], s[NP];
-        if (turns) {
-            const int64_t e = (int64_t)ps * (p.rot / 2) + (HALF ? a0 : a0 / 2);
-            // entries start at a multiple of 4 floats when rot is a multiple of 2V and V of 8, of 2 for V = 4 interleaved
-            load_table<NP>(p.cos_t + e, c, true);
-            load_table<NP>(p.sin_t + e, s, true);
-            if (p.inverse)
-#pragma unroll
-                for (int i = 0; i < NP; i++) s[i] = -s[i];
-        }
-        const T *x = static_cast<const T *>(p.x) + t * p.xt;
-        T *o = static_cast<T *>(p.out) + t * p.ot;
-        float a[kRotHeads][V], b[kRotHeads][V];
-#pragma unroll
-        for (int u = 0; u < kRotHeads; u++) {
-            if (h0 + u >= p.heads) break;
-            const T *xh = x + (h0 + u) * p.xh;
-            load_act<T, V>(xh + a0, a[u], true);
-            if (HALF && turns) load_act<T, V>(xh + b0, b[u], true);
-        }
-#pragma unroll
-        for (int u = 0; u < kRotHeads; u++) {
-            if (h0 + u >= p.heads) break;
-            if (turns) {
-#pragma unroll
-                for (int i = 0; i < NP; i++) {
-                    if constexpr (HALF) turn(a[u][i], b[u][i], c[i], s[i]);
-                    else turn(a[u][2 * i], a[u][2 * i + 1], c[i], s[i]);
-                }
-            }
-            T *oh = o + (h0 + u) * p.oh;
-            store_act<T, V>(oh + a0, a[u], true);
-            if (HALF && turns) store_act<T, V>(oh + b0, b[u], true);
-        }
+        rotary_item<T, HALF>(static_cast<const T *>(p.x) + (int64_t)t * p.xt + h0 * p.xh, p.xh,
+                             static_cast<T *>(p.out) + (int64_t)t * p.ot + h0 * p.oh, p.oh, p.heads - h0, j, p.D, p.rot,
+                             p.cos_t, p.sin_t, p.inverse, [&]() -> int64_t {
+                                 if (ps >= 0 && ps < p.max_seq) return ps;
+                                 atomicExch(&g_rotary_status, VKQ_ERR_INVALID_ARGUMENT);
+                                 return -1;
+                             });
     }
 }
 
-// Any rot, strides and alignment: an item is one pair, or one value past rot.
 template <typename T>
 __global__ void __launch_bounds__(kRotThreads) rotary_any_kernel(const RotaryParams p) {
     pdl_wait();
     pdl_launch_dependents();
-    const int half = p.rot / 2;
     const int64_t stride = (int64_t)gridDim.x * kRotThreads;
     for (int64_t it = (int64_t)blockIdx.x * kRotThreads + threadIdx.x; it < p.items; it += stride) {
         const int64_t th = it / p.pieces;
@@ -119,19 +70,8 @@ __global__ void __launch_bounds__(kRotThreads) rotary_any_kernel(const RotaryPar
             atomicExch(&g_rotary_status, VKQ_ERR_INVALID_ARGUMENT);
             continue;
         }
-        const T *x = static_cast<const T *>(p.x) + t * p.xt + h * p.xh;
-        T *o = static_cast<T *>(p.out) + t * p.ot + h * p.oh;
-        if (j >= half) {
-            o[half + j] = x[half + j];
-            continue;
-        }
-        const int ia = p.half ? j : 2 * j, ib = p.half ? j + half : 2 * j + 1;
-        const int64_t e = (int64_t)ps * half + j;
-        float a = to_f32<T>(x[ia]), b = to_f32<T>(x[ib]);
-        const float s = p.sin_t[e];
-        turn(a, b, p.cos_t[e], p.inverse ? -s : s);
-        o[ia] = from_f32<T>(a);
-        o[ib] = from_f32<T>(b);
+        rotary_one<T>(static_cast<const T *>(p.x) + t * p.xt + h * p.xh, static_cast<T *>(p.out) + t * p.ot + h * p.oh, j,
+                      p.rot, p.half, p.cos_t, p.sin_t, p.inverse, ps);
     }
 }
 
@@ -177,13 +117,15 @@ static cudaError_t launch(const void *fn, int64_t blocks, int threads, void *par
 }
 
 template <typename T>
-static const void *rotary_fn(bool vec, bool half) {
+static const void *rotary_fn(bool vec, bool half, bool small) {
     if (!vec) return (const void *)rotary_any_kernel<T>;
-    return half ? (const void *)rotary_vec_kernel<T, true> : (const void *)rotary_vec_kernel<T, false>;
+    if (small)
+        return half ? (const void *)rotary_vec_kernel<T, true, uint32_t> : (const void *)rotary_vec_kernel<T, false, uint32_t>;
+    return half ? (const void *)rotary_vec_kernel<T, true, int64_t> : (const void *)rotary_vec_kernel<T, false, int64_t>;
 }
 
 cudaError_t rotary(const RotaryArgs &a, cudaStream_t s, int device) {
-    const int size = act_bytes(a.dtype), V = 16 / size;
+    const int size = act_bytes(a.dtype);
     RotaryParams p{};
     p.x = a.x, p.out = a.out, p.cos_t = a.cos_t, p.sin_t = a.sin_t, p.pos = a.positions;
     p.xt = a.x_token, p.xh = a.x_head, p.ot = a.out_token, p.oh = a.out_head;
@@ -193,9 +135,9 @@ cudaError_t rotary(const RotaryArgs &a, cudaStream_t s, int device) {
     // 16-byte pieces: whole ones in every row, pairs (and partners) whole pieces apart
     const uintptr_t bits = (uintptr_t)a.x | (uintptr_t)a.out | (uintptr_t)a.cos_t | (uintptr_t)a.sin_t |
                            (uintptr_t)((a.x_token | a.x_head | a.out_token | a.out_head | a.head_dim) * size);
-    const bool vec = (bits & 15u) == 0 && a.rot_dim % 16 == 0;
+    const bool vec = rotary_vec(bits, a.rot_dim);
     if (vec) {
-        p.pieces = p.half ? p.rot / (2 * V) + (p.D - p.rot) / V : p.D / V;
+        p.pieces = size == 4 ? rotary_pieces<float>(p.D, p.rot, p.half) : rotary_pieces<__half>(p.D, p.rot, p.half);
         p.groups = (p.heads + kRotHeads - 1) / kRotHeads;
         p.items = a.tokens * p.groups * p.pieces;
     } else {
@@ -205,9 +147,10 @@ cudaError_t rotary(const RotaryArgs &a, cudaStream_t s, int device) {
     int64_t blocks = (p.items + kRotThreads - 1) / kRotThreads;
     const int64_t cap = 64 * (int64_t)device_sm_count(device);
     if (blocks > cap) blocks = cap;
-    const void *fn = a.dtype == VKQ_F32   ? rotary_fn<float>(vec, p.half)
-                     : a.dtype == VKQ_F16 ? rotary_fn<__half>(vec, p.half)
-                                          : rotary_fn<__nv_bfloat16>(vec, p.half);
+    const bool small = p.items + blocks * kRotThreads < (int64_t(1) << 32);  // 32-bit item numbers
+    const void *fn = a.dtype == VKQ_F32   ? rotary_fn<float>(vec, p.half, small)
+                     : a.dtype == VKQ_F16 ? rotary_fn<__half>(vec, p.half, small)
+                                          : rotary_fn<__nv_bfloat16>(vec, p.half, small);
     return launch(fn, blocks, kRotThreads, &p, s);
 }
 

@@ -193,12 +193,12 @@ struct Kv8AppendArgs {
     int64_t max_seq, rot_dim;
     int layout;
 };
-// Warps the append's launch needs (the grid's size).
-int64_t kv8_append_warps(const vkq_kv8_cache &c, const vkq_kv8_batch &b, int64_t heads, bool q);
+// CTAs the append's launch needs at most.
+int64_t kv8_append_ctas(const vkq_kv8_cache &c, const vkq_kv8_batch &b, bool q);
 cudaError_t kv8_append(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_batch &b, const Kv8AppendArgs &a,
                        cudaStream_t s);
 cudaError_t kv8_read(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_batch &b, const int *seq, const int *pos,
-                     int64_t n, int dtype, void *k_out, void *v_out, cudaStream_t s, int device);
+                     int64_t n, int dtype, void *k_out, void *v_out, cudaStream_t s);
 int kv8_read_status();
 struct Kv8AttentionArgs {
     int dtype;

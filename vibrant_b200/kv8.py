@@ -19,7 +19,7 @@ import math
 import torch
 
 from . import vkq
-from .tensor import ROPE_LAYOUTS, check_int32, check_tables, dtype_code
+from .tensor import ROPE_LAYOUTS, check_int32, check_tables, dtype_code, stream_of
 
 FORMATS = {"int8": vkq.KV8_INT8, "e4m3": vkq.KV8_E4M3}
 BLOCK = vkq.KV8_BLOCK
@@ -96,19 +96,17 @@ class Cache:
         self._ws: dict[int, torch.Tensor] = {}
         self._need: dict[tuple, int] = {}
 
-    def _stream(self, stream):
-        return stream if stream is not None else torch.cuda.current_stream(self.device)
-
-    def _rows(self, t: torch.Tensor, batch: Batch, heads: int | None, name: str) -> tuple[int, int]:
-        """Pointer and token stride of activations [tokens, heads, head_dim]."""
-        if t.dim() != 3 or t.device != self.device or t.shape[0] != batch.tokens or t.shape[2] != self.head_dim or \
-                (heads is not None and t.shape[1] != heads):
+    def _rows(self, t: torch.Tensor, batch: Batch, heads: int | None, name: str) -> tuple[int, int, int]:
+        """Pointer, token stride and heads of activations [tokens, heads, head_dim]."""
+        s = t.shape
+        if len(s) != 3 or t.device != self.device or s[0] != batch.tokens or s[2] != self.head_dim or \
+                (heads is not None and s[1] != heads):
             raise ValueError(f"{name} must be [{batch.tokens}, {heads or 'heads'}, {self.head_dim}] on {self.device}, "
-                             f"got {tuple(t.shape)} on {t.device}")
-        width = t.shape[1] * t.shape[2]
-        if t.numel() and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2])):
+                             f"got {tuple(s)} on {t.device}")
+        st = t.stride()
+        if s[0] and (st[2] != 1 or (s[1] > 1 and st[1] != s[2])):
             raise ValueError(f"the heads of a token must be contiguous in {name}")
-        return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else width
+        return t.data_ptr(), st[0] if s[0] > 1 else s[1] * s[2], s[1]
 
     def append(self, layer: int, batch: Batch, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None = None,
                cos: torch.Tensor | None = None, sin: torch.Tensor | None = None, layout: str = "interleaved",
@@ -117,8 +115,8 @@ class Cache:
         the pages of `layer`; with tables k is rotated first, and q [tokens,
         heads, head_dim] is returned rotated (q_out may be q)."""
         code = dtype_code(k)
-        kp, ks = self._rows(k, batch, self.kv_heads, "k")
-        vp, vs = self._rows(v, batch, self.kv_heads, "v")
+        kp, ks, _ = self._rows(k, batch, self.kv_heads, "k")
+        vp, vs, _ = self._rows(v, batch, self.kv_heads, "v")
         if v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
             raise ValueError("q, k and v must have one dtype")
         if (cos is None) != (sin is None) or (q is not None and cos is None):
@@ -128,18 +126,17 @@ class Cache:
             check_tables(cos, sin, self.device)
             seq, rot = cos.shape[0], 2 * cos.shape[1]
         if q is not None:
-            qp, qs = self._rows(q, batch, None, "q")
-            heads = q.shape[1]
+            qp, qs, heads = self._rows(q, batch, None, "q")
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+                q_out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
             elif q_out.dtype != q.dtype:
                 raise ValueError("q_out must match q")
-            qop, qos = self._rows(q_out, batch, heads, "q_out")
+            qop, qos, _ = self._rows(q_out, batch, heads, "q_out")
         if batch.tokens == 0:
             return q_out
         vkq.kv8_append(self.struct, layer, batch.bounds(self.page_size), code, kp, ks, vp, vs, qp or None, qs,
                        qop or None, qos, heads, _ptr(cos), _ptr(sin), seq, rot, ROPE_LAYOUTS[layout],
-                       device=self.device.index, stream=self._stream(stream))
+                       device=self.device.index, stream=stream_of(self.device, stream))
         return q_out
 
     def read(self, layer: int, batch: Batch, seq: torch.Tensor, pos: torch.Tensor, dtype=torch.float32,
@@ -147,12 +144,14 @@ class Cache:
         """K and V [n, kv_heads, head_dim] of sequence seq[i] of the batch at position pos[i]."""
         check_int32(seq, (None,), "seq", self.device)
         check_int32(pos, (seq.shape[0],), "pos", self.device)
-        out = torch.empty((2, seq.shape[0], self.kv_heads, self.head_dim), dtype=dtype, device=self.device)
-        if seq.shape[0]:
-            vkq.kv8_read(self.struct, layer, batch.bounds(self.page_size), seq.data_ptr(), pos.data_ptr(),
-                         seq.shape[0], dtype_code(out), out[0].data_ptr(), out[1].data_ptr(),
-                         device=self.device.index, stream=self._stream(stream))
-        return out[0], out[1]
+        n = seq.shape[0]
+        shape = (n, self.kv_heads, self.head_dim)
+        k, v = torch.empty(shape, dtype=dtype, device=self.device), torch.empty(shape, dtype=dtype, device=self.device)
+        if n:
+            vkq.kv8_read(self.struct, layer, batch.bounds(self.page_size), seq.data_ptr(), pos.data_ptr(), n,
+                         dtype_code(k), k.data_ptr(), v.data_ptr(), device=self.device.index,
+                         stream=stream_of(self.device, stream))
+        return k, v
 
     def workspace_bytes(self, batch: Batch, dtype: torch.dtype, heads: int, causal: bool = True, window: int = 0) -> int:
         """vkq_kv8_attention_workspace_bytes, memoised."""
@@ -166,16 +165,17 @@ class Cache:
             self._need[key] = need
         return need
 
-    def _workspace(self, nbytes: int, stream) -> torch.Tensor:
+    def _workspace(self, nbytes: int, stream: torch.cuda.Stream | None) -> torch.Tensor:
         """A zero-filled workspace of this cache and stream (calls on one stream may share it)."""
-        ws = self._ws.get(stream.cuda_stream)
+        key = stream_of(self.device, stream)
+        ws = self._ws.get(key)
         if ws is None or ws.numel() < nbytes:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("the workspace cannot grow in a stream capture: make the call once before, or "
                                    "give ws (zero-filled, workspace_bytes(...) long)")
-            with torch.cuda.stream(stream):
+            with torch.cuda.stream(stream):  # None: the current one
                 ws = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=self.device)
-            self._ws[stream.cuda_stream] = ws
+            self._ws[key] = ws
         return ws
 
     def attend(self, layer: int, batch: Batch, q: torch.Tensor, scale: float | None = None, causal: bool = True,
@@ -184,22 +184,19 @@ class Cache:
         """Attention of the new tokens' q [tokens, heads, head_dim] over the
         cache (which holds them already); scale defaults to 1 / sqrt(head_dim)."""
         code = dtype_code(q)
-        qp, qs = self._rows(q, batch, None, "q")
-        heads = q.shape[1]
+        qp, qs, heads = self._rows(q, batch, None, "q")
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
         elif out.dtype != q.dtype:
             raise ValueError("out must match q")
-        op, os_ = self._rows(out, batch, heads, "out")
+        op, os_, _ = self._rows(out, batch, heads, "out")
         if batch.tokens == 0:
             return out
-        st = self._stream(stream)
-        need = self.workspace_bytes(batch, q.dtype, heads, causal, window)
         if ws is None:
-            ws = self._workspace(need, st)
+            ws = self._workspace(self.workspace_bytes(batch, q.dtype, heads, causal, window), stream)
         vkq.kv8_attention(self.struct, layer, batch.bounds(self.page_size), code, qp, qs, op, os_, heads,
                           1.0 / math.sqrt(self.head_dim) if scale is None else scale, ws.data_ptr(), ws.numel(),
-                          causal, window, device=self.device.index, stream=st)
+                          causal, window, device=self.device.index, stream=stream_of(self.device, stream))
         return out
 
     def copy_pages(self, src: torch.Tensor, dst: torch.Tensor, stream: torch.cuda.Stream | None = None) -> None:
@@ -208,7 +205,7 @@ class Cache:
         check_int32(dst, (src.shape[0],), "dst", self.device)
         if src.shape[0]:
             vkq.kv8_copy_pages(self.struct, src.data_ptr(), dst.data_ptr(), src.shape[0], device=self.device.index,
-                               stream=self._stream(stream))
+                               stream=stream_of(self.device, stream))
 
 
 class Sequences:
@@ -249,7 +246,7 @@ class Sequences:
         if n:
             vkq.kv8_extend(self.cache.struct, self.struct, slots.data_ptr(), add.data_ptr(), n, _ptr(done),
                            self._ws.data_ptr(), self._ws.numel(), device=self.cache.device.index,
-                           stream=self.cache._stream(stream))
+                           stream=stream_of(self.cache.device, stream))
 
     def fork(self, src: torch.Tensor, dst: torch.Tensor, done: torch.Tensor | None = None, stream=None) -> None:
         """The empty rows dst become copies of the rows src: whole pages shared, a part-filled last one copied."""
@@ -258,18 +255,18 @@ class Sequences:
         if n:
             vkq.kv8_fork(self.cache.struct, self.struct, src.data_ptr(), dst.data_ptr(), n, _ptr(done),
                          self._ws.data_ptr(), self._ws.numel(), device=self.cache.device.index,
-                         stream=self.cache._stream(stream))
+                         stream=stream_of(self.cache.device, stream))
 
     def free(self, slots: torch.Tensor, done: torch.Tensor | None = None, stream=None) -> None:
         """The listed rows become empty; pages that no row holds any more are free."""
         n = self._list(slots, "slots", done)
         if n:
             vkq.kv8_free(self.cache.struct, self.struct, slots.data_ptr(), n, _ptr(done), self._ws.data_ptr(),
-                         self._ws.numel(), device=self.cache.device.index, stream=self.cache._stream(stream))
+                         self._ws.numel(), device=self.cache.device.index, stream=stream_of(self.cache.device, stream))
 
     def compact(self, used: torch.Tensor | None = None, stream=None) -> None:
         """The pages in use become pages 0 .. used - 1, their contents moved and the table renamed."""
         if used is not None:
             check_int32(used, (1,), "used", self.cache.device)
         vkq.kv8_compact(self.cache.struct, self.struct, _ptr(used), self._ws.data_ptr(), self._ws.numel(),
-                        device=self.cache.device.index, stream=self.cache._stream(stream))
+                        device=self.cache.device.index, stream=stream_of(self.cache.device, stream))

@@ -141,16 +141,17 @@ def dtype_code(t: torch.Tensor) -> int:
         raise ValueError(f"float32, float16 or bfloat16 needed, got {t.dtype}") from None
 
 
-def _device_index(t: torch.Tensor) -> int:
-    if not t.is_cuda:
-        raise ValueError("a CUDA tensor is needed")
-    return t.device.index
+def stream_of(device: torch.device, stream: torch.cuda.Stream | None) -> int:
+    """The stream's handle, torch's current one by default (asked for as a
+    handle: a call's host time counts where the kernel takes a microsecond)."""
+    return torch._C._cuda_getCurrentRawStream(device.index) if stream is None else stream.cuda_stream
 
 
 def check_int32(t: torch.Tensor, shape: tuple, name: str, device: torch.device) -> None:
     """An int32 contiguous tensor of that shape (None: any extent) on the device."""
-    if t.dtype != torch.int32 or t.device != device or not t.is_contiguous() or t.dim() != len(shape) or \
-            any(n is not None and n != m for n, m in zip(shape, t.shape)):
+    s = t.shape
+    if t.dtype != torch.int32 or t.device != device or not t.is_contiguous() or len(s) != len(shape) or \
+            (s != shape and any(n is not None and n != m for n, m in zip(shape, s))):
         raise ValueError(f"{name} must be a contiguous int32 tensor of shape {shape} on {device}, got "
                          f"{tuple(t.shape)} {t.dtype} on {t.device}")
 
@@ -168,9 +169,8 @@ def rotary_tables(rot_dim: int, base: float, max_seq: int, scaling: str = "none"
     (vkq_rotary_tables_f32); scaling "none", "linear", "ntk" or "yarn"."""
     cos = torch.empty((max_seq, rot_dim // 2), dtype=torch.float32, device=device)
     sin = torch.empty_like(cos)
-    st = stream if stream is not None else torch.cuda.current_stream(cos.device)
     vkq.rotary_tables_f32(cos.data_ptr(), sin.data_ptr(), max_seq, rot_dim, base, ROPE_SCALINGS[scaling], factor,
-                          orig_len, beta_fast, beta_slow, attn_factor, device=cos.device.index, stream=st)
+                          orig_len, beta_fast, beta_slow, attn_factor, device=cos.device.index, stream=stream_of(cos.device, stream))
     return cos, sin
 
 
@@ -179,22 +179,28 @@ def rotary(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: tor
            stream: torch.cuda.Stream | None = None) -> torch.Tensor:
     """Rotary positions of x [tokens, heads, head_dim] (any token and head
     strides) by the tables' rows positions[t] (vkq_rotary); out may be x."""
-    if x.dim() != 3 or x.stride(2) != 1 and x.shape[2] > 1:
-        raise ValueError("x must be [tokens, heads, head_dim] with contiguous heads")
-    dev = _device_index(x)
-    check_tables(cos, sin, x.device)
-    check_int32(positions, (x.shape[0],), "positions", x.device)
+    if x.dim() != 3:
+        raise ValueError("x must be [tokens, heads, head_dim]")
+    (T, H, D), xs, dev = x.shape, x.stride(), x.device
+    if xs[2] != 1 and D > 1:
+        raise ValueError("the values of a head must be contiguous")
+    if dev.type != "cuda":
+        raise ValueError("a CUDA tensor is needed")
+    check_tables(cos, sin, dev)
+    check_int32(positions, (T,), "positions", dev)
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or out.stride(2) != 1:
-        raise ValueError("out must match x")
+        out = torch.empty((T, H, D), dtype=x.dtype, device=dev)
+        os_ = (H * D, D, 1)
+    else:
+        os_ = out.stride()
+        if out.shape != x.shape or out.dtype != x.dtype or out.device != dev or (os_[2] != 1 and D > 1):
+            raise ValueError("out must match x")
     if x.numel() == 0:
         return out
-    st = stream if stream is not None else torch.cuda.current_stream(x.device)
-    T, H, D = x.shape
-    vkq.rotary(dtype_code(x), x.data_ptr(), (x.stride(0), x.stride(1)), out.data_ptr(),
-               (out.stride(0), out.stride(1)), cos.data_ptr(), sin.data_ptr(), positions.data_ptr(), T, H, D,
-               2 * cos.shape[1], cos.shape[0], ROPE_LAYOUTS[layout], inverse, device=dev, stream=st)
+    rows, half = cos.shape
+    vkq.rotary(dtype_code(x), x.data_ptr(), xs, out.data_ptr(), os_, cos.data_ptr(), sin.data_ptr(),
+               positions.data_ptr(), T, H, D, 2 * half, rows, ROPE_LAYOUTS[layout], inverse, device=dev.index,
+               stream=stream_of(dev, stream))
     return out
 
 

@@ -162,9 +162,7 @@ def weight_bytes(qtype: int, K: int, N: int) -> int:
 
 
 def _stream_ptr(stream) -> int | None:
-    if stream is None:
-        return None
-    if isinstance(stream, int):
+    if stream is None or isinstance(stream, int):
         return stream
     return stream.cuda_stream  # torch.cuda.Stream
 
@@ -305,7 +303,7 @@ def rotary(dtype: int, x_ptr: int, x_strides: tuple[int, int], out_ptr: int, out
     given (token, head) strides, in elements."""
     _check(load().vkq_rotary(device, dtype, x_ptr, x_strides[0], x_strides[1], out_ptr, out_strides[0],
                              out_strides[1], cos_ptr, sin_ptr, pos_ptr, tokens, heads, head_dim, rot_dim, max_seq,
-                             layout, int(inverse), _stream_ptr(stream)))
+                             layout, inverse, _stream_ptr(stream)))
 
 
 def rotary_tables_f32(cos_ptr: int, sin_ptr: int, max_seq: int, rot_dim: int, base: float,
