@@ -101,6 +101,20 @@ __device__ __forceinline__ uint32_t kv8_encode(float x, bool e4m3) {
     if (e4m3) return __nv_cvt_float_to_fp8(fminf(fmaxf(x, -448.f), 448.f), __NV_SATFINITE, __NV_E4M3);
     return (uint32_t)(uint8_t)(int8_t)__float2int_rn(fminf(fmaxf(x, -127.f), 127.f));
 }
+// Four codes of values within the format's range (finite, |x| <= 448 or 127).
+__device__ __forceinline__ uint32_t kv8_encode4(float a, float b, float c, float d, bool e4m3) {
+    if (e4m3) {
+        uint16_t lo, hi;
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+        return (uint32_t)lo | ((uint32_t)hi << 16);
+    }
+    // adding 1.5 * 2^23 leaves the integer (ties to even) in the low bits
+    const float m = 12582912.f;
+    const uint32_t x = __float_as_uint(__fadd_rn(a, m)), y = __float_as_uint(__fadd_rn(b, m));
+    const uint32_t z = __float_as_uint(__fadd_rn(c, m)), w = __float_as_uint(__fadd_rn(d, m));
+    return prmt(prmt(x, y, 0x0040u), prmt(z, w, 0x0040u), 0x5410u);
+}
 // The least power of two s in [2^-64, 2^63] with a <= m * s (a finite, >= 0).
 __device__ __forceinline__ float kv8_scale(float a, bool e4m3) {
     const float m = e4m3 ? 448.f : 127.f;

@@ -239,7 +239,7 @@ int vkq_kv8_append(int device, const vkq_kv8_cache *cache, int64_t layer, const 
     }
     Kv8AppendArgs a{dtype,     k,         v,       q,       k_token_stride, v_token_stride, q_token_stride, q_out, q_out_token_stride,
                     heads, cos_table, sin_table, max_seq, rot_dim, layout};
-    return check_launch(kv8_append(*cache, layer, *batch, a, (cudaStream_t)stream), "KV cache append");
+    return check_launch(kv8_append(*cache, layer, *batch, a, (cudaStream_t)stream, device), "KV cache append");
 }
 
 int vkq_kv8_read(int device, const vkq_kv8_cache *cache, int64_t layer, const vkq_kv8_batch *batch, const int32_t *seq,

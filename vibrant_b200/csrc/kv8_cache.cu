@@ -12,9 +12,9 @@
 // last scale (with free scales, 15 appends could add 15 half steps).  The cost
 // is up to one bit of the int8 code's range; e4m3 loses nothing.
 //
-// One CTA takes one block of K or V: four rows a warp (D / 32 values of a row a
-// lane), the maximum over the warps through shared memory.  No other CTA
-// touches the block, so there are no atomics and the result does not depend on
+// A CTA takes K or V of one head of a block, or one after another of all heads:
+// four rows a warp (D / 32 values of a row a lane), the maximum over the warps
+// through shared memory.  No other CTA touches its items, so there are no atomics and the result does not depend on
 // the order of anything.  Bytes bound a prompt, latency a decode step; q's
 // rotation rides in the same launch (CTAs past the blocks', a few tokens each),
 // which saves a launch a layer.
@@ -48,7 +48,9 @@ struct AppendParams {
     int64_t max_seq;
     int heads, rot;
     uint32_t max_blocks;   // blocks that one sequence's new tokens can touch
-    uint32_t block_ctas;   // batch * max_blocks * kv_heads * 2
+    int items;             // (K or V, head) of a block that a CTA takes, and the CTAs that this makes
+    uint32_t groups, block_ctas;  // block_ctas = batch * max_blocks * groups
+    uint32_t magic_groups, magic_blocks, magic_page;  // of groups, max_blocks, page / 16 (kv8_div)
     int q_tokens, q_items; // tokens of a CTA of q's, items of a token
     bool half, vec_kv, vec_t, vec_q;  // a lane's values as one vector: k and v, the tables; q by 16-byte pieces
 };
@@ -76,6 +78,9 @@ __device__ __forceinline__ void load_entries(const AppendParams &p, const LaneTu
         const int64_t e = row + (l.d0 < l.h ? l.d0 : l.d0 - l.h);
         load_act<float, N>(p.cos_t + e, c, true);
         load_act<float, N>(p.sin_t + e, s, true);
+        if (l.d0 < l.h)
+#pragma unroll
+            for (int i = 0; i < N; i++) s[i] = -s[i];
     } else {
         float a[N / 2], b[N / 2];
         if constexpr (N == 4) {
@@ -89,12 +94,37 @@ __device__ __forceinline__ void load_entries(const AppendParams &p, const LaneTu
         for (int i = 0; i < N / 2; i++) c[i] = a[i], s[i] = b[i];
     }
 }
-// The lane's values x of `row` and their partners y (half, vec).
+// N elements as they are in memory, in words.
 template <typename T, int N>
-__device__ __forceinline__ void load_pair(const T *row, const LaneTurn &l, bool vec, float (&x)[N], float (&y)[N]) {
-    load_act<T, N>(row + l.d0, x, vec);
-    if (l.rotate && l.vec && l.half && l.d0 < l.rot) load_act<T, N>(row + (l.d0 < l.h ? l.d0 + l.h : l.d0 - l.h), y, vec);
-}
+struct Raw {
+    static constexpr int W = N * (int)sizeof(T) / 4;  // 1, 2 or 4
+    uint32_t w[W];
+    __device__ __forceinline__ void load(const T *p, bool vec) {
+        if (vec) {
+            if constexpr (W == 4) {
+                const uint4 x = *reinterpret_cast<const uint4 *>(p);
+                w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+            } else if constexpr (W == 2) {
+                const uint2 x = *reinterpret_cast<const uint2 *>(p);
+                w[0] = x.x, w[1] = x.y;
+            } else {
+                w[0] = *reinterpret_cast<const uint32_t *>(p);
+            }
+        } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < W; i++) w[i] = *reinterpret_cast<const uint32_t *>(p + i);
+        } else {
+            const uint16_t *h = reinterpret_cast<const uint16_t *>(p);
+#pragma unroll
+            for (int i = 0; i < W; i++) w[i] = (uint32_t)h[2 * i] | ((uint32_t)h[2 * i + 1] << 16);
+        }
+    }
+    __device__ __forceinline__ void get(float (&x)[N]) const {
+        const T *v = reinterpret_cast<const T *>(w);
+#pragma unroll
+        for (int i = 0; i < N; i++) x[i] = to_f32<T>(v[i]);
+    }
+};
 template <typename T, int N>
 __device__ __forceinline__ void turn_lane(const AppendParams &p, const T *row, const LaneTurn &l, int64_t ps,
                                           const float (&c)[N], const float (&s)[N], float (&x)[N], float (&y)[N]) {
@@ -102,10 +132,8 @@ __device__ __forceinline__ void turn_lane(const AppendParams &p, const T *row, c
     if (l.vec) {
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            if (l.half) {
-                float a = l.d0 < l.h ? x[i] : y[i], b = l.d0 < l.h ? y[i] : x[i];
-                turn(a, b, c[i], s[i]);
-                x[i] = l.d0 < l.h ? a : b;
+            if (l.half) {  // s of the first half comes negated: x c - y s is x c + y (-s)
+                x[i] = __fadd_rn(__fmul_rn(x[i], c[i]), __fmul_rn(y[i], s[i]));
             } else if (i % 2 == 0) {
                 turn(x[i], x[i + 1], c[i / 2], s[i / 2]);
             }
@@ -131,15 +159,15 @@ __device__ __forceinline__ void turn_lane(const AppendParams &p, const T *row, c
 template <typename T, int D>
 __device__ void append_block(const AppendParams &p, uint32_t cta) {
     constexpr int N = D / 32;
-    __shared__ float amax[kAppWarps];
+    __shared__ float amax[2][kAppWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const bool is_v = cta & 1;
-    uint32_t r = cta >> 1;
-    const uint32_t kvh = (uint32_t)p.pool.kv_heads;
-    const int h = (int)(r % kvh);
-    r /= kvh;
-    const int j = (int)(r % p.max_blocks);
-    const Kv8Seq s = kv8_seq(p.batch, p.pool.page, r / p.max_blocks);
+    const int kvh = p.pool.kv_heads;
+    // the CTA's block, and which of its items (the K heads, then the V heads)
+    const uint32_t r = kv8_div(cta, p.groups, p.magic_groups);
+    const int i0 = (int)(cta - r * p.groups) * p.items, i1 = min(i0 + p.items, 2 * kvh);
+    const uint32_t seq = kv8_div(r, p.max_blocks, p.magic_blocks);
+    const int j = (int)(r - seq * p.max_blocks);
+    const Kv8Seq s = kv8_seq(p.batch, p.pool.page, seq);
     const bool rotate = p.cos_t != nullptr;
     if (!s.ok || s.n > s.len || (rotate && s.len > p.max_seq)) {
         if (threadIdx.x == 0 && j == 0) kv8_bad();
@@ -149,68 +177,111 @@ __device__ void append_block(const AppendParams &p, uint32_t cta) {
     const int pos0 = (start / kKv8Block + j) * kKv8Block;
     if (s.n == 0 || pos0 >= s.len) return;
     const int lo = max(start - pos0, 0), hi = min(s.len - pos0, kKv8Block);  // the block's new rows
-    const T *src = static_cast<const T *>(is_v ? p.v : p.k) + (int64_t)(s.first + pos0 - start) * (is_v ? p.vt : p.kt) +
-                   h * D;
-    const int64_t stride = is_v ? p.vt : p.kt;
-    const LaneTurn lt = lane_turn<N>(p, lane, rotate && !is_v);
-    float x[kAppRows][N], y[kAppRows][N], c[kAppRows][N], sn[kAppRows][N];
+    const int64_t row0 = (int64_t)(s.first + pos0 - start);
+    const LaneTurn lt_k = lane_turn<N>(p, lane, rotate), lt_v = lane_turn<N>(p, lane, false);
+    const bool pairs = lt_k.rotate && lt_k.vec && lt_k.half && lt_k.d0 < lt_k.rot;
+    const int partner = lt_k.d0 < lt_k.h ? lt_k.d0 + lt_k.h : lt_k.d0 - lt_k.h;
+    // the rows of an item; the next item's are under way while one is worked on
+    Raw<T, N> xr[kAppRows], yr[kAppRows];
+    auto load = [&](int it) {
+        const bool is_v = it >= kvh;
+        const int64_t stride = is_v ? p.vt : p.kt;
+        const T *src = static_cast<const T *>(is_v ? p.v : p.k) + row0 * stride + (is_v ? it - kvh : it) * D;
+#pragma unroll
+        for (int i = 0; i < kAppRows; i++) {
+            const int t = warp + i * kAppWarps;
+            if (t < lo || t >= hi) continue;
+            xr[i].load(src + t * stride + lane * N, p.vec_kv);
+            if (pairs && !is_v) yr[i].load(src + t * stride + partner, p.vec_kv);
+        }
+    };
+    load(i0);
+    float c[kAppRows][N], sn[kAppRows][N];  // all K heads turn alike
 #pragma unroll
     for (int i = 0; i < kAppRows; i++) {
         const int t = warp + i * kAppWarps;
-        if (t < lo || t >= hi) continue;
-        load_pair<T, N>(src + t * stride, lt, p.vec_kv, x[i], y[i]);
-        load_entries<N>(p, lt, pos0 + t, c[i], sn[i]);
+        if (t >= lo && t < hi && i0 < kvh) load_entries<N>(p, lt_k, pos0 + t, c[i], sn[i]);
     }
-    const int id = kv8_page(p.pool, s, pos0 / p.pool.page);
+    const uint32_t per_page = (uint32_t)(p.pool.page / kKv8Block), blk = (uint32_t)(pos0 / kKv8Block);
+    const uint32_t lp = kv8_div(blk, per_page, p.magic_page);
+    const int id = kv8_page(p.pool, s, (int)lp);
     if (id < 0) {
         if (threadIdx.x == 0) kv8_bad();
         return;
     }
-    const int in_page = pos0 % p.pool.page;
-    const int64_t ph = (int64_t)id * kvh + h;
-    float *scale = (is_v ? p.pool.vs : p.pool.ks) + ph * (p.pool.page / kKv8Block) + in_page / kKv8Block;
-    uint8_t *codes = (is_v ? p.pool.v : p.pool.k) + (ph * p.pool.page + in_page) * D + lane * N;
-    const float s_old = lo > 0 ? *scale : 0.f;
-    float a = 0.f;
+    const int64_t at0 = (int64_t)id * kvh * per_page + (blk - lp * per_page);
+#pragma unroll 1
+    for (int it = i0; it < i1; it++) {
+        const bool is_v = it >= kvh;
+        const int h = is_v ? it - kvh : it;
+        const int64_t at = at0 + (int64_t)h * per_page, stride = is_v ? p.vt : p.kt;
+        float *scale = (is_v ? p.pool.vs : p.pool.ks) + at;
+        uint8_t *codes = (is_v ? p.pool.v : p.pool.k) + at * (kKv8Block * D) + lane * N;
+        const T *src = static_cast<const T *>(is_v ? p.v : p.k) + row0 * stride + h * D;
+        const float s_old = lo > 0 ? *scale : 0.f;
+        float x[kAppRows][N];
+        float a = 0.f, z = 0.f;  // z: 0, or NaN after a value that is no number or infinite
 #pragma unroll
-    for (int i = 0; i < kAppRows; i++) {
-        const int t = warp + i * kAppWarps;
-        if (t < lo || t >= hi) continue;
-        turn_lane<T, N>(p, src + t * stride, lt, pos0 + t, c[i], sn[i], x[i], y[i]);
+        for (int i = 0; i < kAppRows; i++) {
+            const int t = warp + i * kAppWarps;
+            if (t < lo || t >= hi) continue;
+            float y[N];
+            xr[i].get(x[i]);
+            yr[i].get(y);
+            turn_lane<T, N>(p, src + t * stride, is_v ? lt_v : lt_k, pos0 + t, c[i], sn[i], x[i], y);
 #pragma unroll
-        for (int u = 0; u < N; u++) {
-            const float m = fabsf(x[i][u]);
-            if (m <= 3.402823466e38f) a = fmaxf(a, m);  // finite
+            for (int u = 0; u < N; u++) {
+                a = fmaxf(a, fabsf(x[i][u]));
+                z = fmaf(x[i][u], 0.f, z);
+            }
         }
-    }
+        if (it + 1 < i1) load(it + 1);
+        const bool odd = __syncthreads_or(!(z == 0.f));
+        if (odd) {  // the largest of the finite ones
+            a = 0.f;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-    if (lane == 0) amax[warp] = a;
-    __syncthreads();  // every thread has read the old scale, too
+            for (int i = 0; i < kAppRows; i++) {
+                const int t = warp + i * kAppWarps;
 #pragma unroll
-    for (int w = 0; w < kAppWarps; w++) a = fmaxf(a, amax[w]);
-    const float sc = fmaxf(s_old, kv8_scale(a, p.pool.e4m3));
-    const bool grew = lo > 0 && sc > s_old;
-    const float inv = __fdiv_rn(1.f, sc), ratio = grew ? __fdiv_rn(s_old, sc) : 1.f;
-#pragma unroll
-    for (int i = 0; i < kAppRows; i++) {
-        const int t = warp + i * kAppWarps;
-        if (t >= hi || (t < lo && !grew)) continue;
-        uint8_t *out = codes + t * D;
-        uint32_t o = 0;
-        if (t < lo) {
-            const uint32_t w = N == 4 ? *reinterpret_cast<uint32_t *>(out) : *reinterpret_cast<uint16_t *>(out);
-#pragma unroll
-            for (int u = 0; u < N; u++)
-                o |= kv8_encode(kv8_decode((w >> (8 * u)) & 0xFFu, p.pool.e4m3) * ratio, p.pool.e4m3) << (8 * u);
-        } else {
-#pragma unroll
-            for (int u = 0; u < N; u++) o |= kv8_encode(x[i][u] * inv, p.pool.e4m3) << (8 * u);
+                for (int u = 0; u < N; u++)
+                    if (t >= lo && t < hi && fabsf(x[i][u]) <= 3.402823466e38f) a = fmaxf(a, fabsf(x[i][u]));
+            }
         }
-        if (N == 4) *reinterpret_cast<uint32_t *>(out) = o;
-        else *reinterpret_cast<uint16_t *>(out) = (uint16_t)o;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+        if (lane == 0) amax[it & 1][warp] = a;
+        __syncthreads();  // every thread has read the old scale, too
+#pragma unroll
+        for (int w = 0; w < kAppWarps; w++) a = fmaxf(a, amax[it & 1][w]);
+        const float sc = fmaxf(s_old, kv8_scale(a, p.pool.e4m3));
+        const bool grew = lo > 0 && sc > s_old;
+        const uint32_t bits = __float_as_uint(sc);  // of a power of two: the inverse is one subtraction
+        const float inv = (bits & 0x7fffffu) == 0 ? __uint_as_float(0x7f000000u - bits) : __fdiv_rn(1.f, sc);
+        const float ratio = grew ? __fdiv_rn(s_old, sc) : 1.f;
+        const bool saturates = odd || sc >= kKv8MaxScale;
+#pragma unroll
+        for (int i = 0; i < kAppRows; i++) {
+            const int t = warp + i * kAppWarps;
+            if (t >= hi || (t < lo && !grew)) continue;
+            uint8_t *out = codes + t * D;
+            uint32_t o = 0;
+            if (t < lo) {
+                const uint32_t w = N == 4 ? *reinterpret_cast<uint32_t *>(out) : *reinterpret_cast<uint16_t *>(out);
+#pragma unroll
+                for (int u = 0; u < N; u++)
+                    o |= kv8_encode(kv8_decode((w >> (8 * u)) & 0xFFu, p.pool.e4m3) * ratio, p.pool.e4m3) << (8 * u);
+            } else if (saturates) {
+#pragma unroll
+                for (int u = 0; u < N; u++) o |= kv8_encode(x[i][u] * inv, p.pool.e4m3) << (8 * u);
+            } else {
+                o = kv8_encode4(x[i][0] * inv, x[i][1] * inv, N == 4 ? x[i][N - 2] * inv : 0.f,
+                                N == 4 ? x[i][N - 1] * inv : 0.f, p.pool.e4m3);
+            }
+            if (N == 4) *reinterpret_cast<uint32_t *>(out) = o;
+            else *reinterpret_cast<uint16_t *>(out) = (uint16_t)o;
+        }
+        if (threadIdx.x == 0) *scale = sc;
     }
-    if (threadIdx.x == 0) *scale = sc;
 }
 
 // The sequence of token t: the last b with cu[b] <= t (empty sequences skipped).
@@ -262,7 +333,7 @@ __device__ void append_q(const AppendParams &p, uint32_t cta) {
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kAppThreads) append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kAppThreads, 6) append_kernel(const AppendParams p) {
     pdl_wait();
     pdl_launch_dependents();
     if (blockIdx.x < p.block_ctas) append_block<T, D>(p, blockIdx.x);
@@ -315,26 +386,33 @@ __global__ void __launch_bounds__(kReadThreads) read_kernel(const ReadParams p) 
     const int quads = D / 4, width = p.pool.kv_heads * quads, rows = (int)min((int64_t)p.rows, p.n - r0);
     for (int x = threadIdx.x; x < width; x += kReadThreads) {
         const int h = x / quads, d = (x - h * quads) * 4;
+        uint32_t kw[kReadRows], vw[kReadRows];
+        float ks[kReadRows], vs[kReadRows];
+#pragma unroll
+        for (int i = 0; i < kReadRows; i++) {
+            if (i < rows && row_at[i] >= 0) {
+                const int64_t e = row_at[i] + (int64_t)h * page * D + d, se = scale_at[i] + h * (page / kKv8Block);
+                kw[i] = *reinterpret_cast<const uint32_t *>(p.pool.k + e);
+                vw[i] = *reinterpret_cast<const uint32_t *>(p.pool.v + e);
+                ks[i] = p.pool.ks[se], vs[i] = p.pool.vs[se];
+            } else {
+                kw[i] = vw[i] = 0;
+                ks[i] = vs[i] = __int_as_float(0x7fc00000);
+            }
+        }
 #pragma unroll
         for (int i = 0; i < kReadRows; i++) {
             if (i >= rows) break;
             float kx[4], vx[4];
-            if (row_at[i] < 0) {
-                kx[0] = kx[1] = kx[2] = kx[3] = vx[0] = vx[1] = vx[2] = vx[3] = __int_as_float(0x7fc00000);
-            } else {
-                const int64_t e = row_at[i] + (int64_t)h * page * D + d, se = scale_at[i] + h * (page / kKv8Block);
-                const uint32_t kw = kv8_unsign<E4M3>(*reinterpret_cast<const uint32_t *>(p.pool.k + e));
-                const uint32_t vw = kv8_unsign<E4M3>(*reinterpret_cast<const uint32_t *>(p.pool.v + e));
-                const float ks = p.pool.ks[se], vs = p.pool.vs[se];
-                const uint32_t w[4] = {kv8_widen<E4M3, false>(kw), kv8_widen<E4M3, true>(kw), kv8_widen<E4M3, false>(vw),
-                                       kv8_widen<E4M3, true>(vw)};
+            const uint32_t kb = kv8_unsign<E4M3>(kw[i]), vb = kv8_unsign<E4M3>(vw[i]);
+            const uint32_t w[4] = {kv8_widen<E4M3, false>(kb), kv8_widen<E4M3, true>(kb), kv8_widen<E4M3, false>(vb),
+                                   kv8_widen<E4M3, true>(vb)};
 #pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&w[u]));
-                    const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&w[2 + u]));
-                    kx[2 * u] = a.x * ks, kx[2 * u + 1] = a.y * ks;
-                    vx[2 * u] = b.x * vs, vx[2 * u + 1] = b.y * vs;
-                }
+            for (int u = 0; u < 2; u++) {
+                const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&w[u]));
+                const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&w[2 + u]));
+                kx[2 * u] = a.x * ks[i], kx[2 * u + 1] = a.y * ks[i];
+                vx[2 * u] = b.x * vs[i], vx[2 * u + 1] = b.y * vs[i];
             }
             const int64_t o = (r0 + i) * width * 4 + x * 4;
             if (p.k_out) store_act<T, 4>(static_cast<T *>(p.k_out) + o, kx, true);
@@ -362,15 +440,13 @@ static const void *append_fn(int D) {
     return D == 64 ? (const void *)append_kernel<T, 64> : (const void *)append_kernel<T, 128>;
 }
 
-static int64_t append_blocks(const vkq_kv8_cache &c, const vkq_kv8_batch &b) {
-    return b.batch * ((b.max_tokens + kKv8Block - 2) / kKv8Block + 1) * c.kv_heads * 2;
-}
+static int64_t append_max_blocks(const vkq_kv8_batch &b) { return (b.max_tokens + kKv8Block - 2) / kKv8Block + 1; }
 int64_t kv8_append_ctas(const vkq_kv8_cache &c, const vkq_kv8_batch &b, bool q) {
-    return append_blocks(c, b) + (q ? b.tokens : 0);
+    return b.batch * append_max_blocks(b) * c.kv_heads * 2 + (q ? b.tokens : 0);
 }
 
 cudaError_t kv8_append(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_batch &b, const Kv8AppendArgs &a,
-                       cudaStream_t s) {
+                       cudaStream_t s, int device) {
     AppendParams p{};
     p.pool = kv8_pool(c, layer);
     p.batch = kv8_batch(b);
@@ -378,8 +454,15 @@ cudaError_t kv8_append(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_batc
     p.kt = a.k_token, p.vt = a.v_token, p.qt = a.q_token, p.qot = a.q_out_token;
     p.cos_t = a.cos_t, p.sin_t = a.sin_t, p.max_seq = a.max_seq;
     p.heads = (int)a.heads, p.rot = (int)a.rot_dim, p.half = a.layout == VKQ_ROPE_HALF;
-    p.max_blocks = (uint32_t)((b.max_tokens + kKv8Block - 2) / kKv8Block + 1);
-    p.block_ctas = (uint32_t)append_blocks(c, b);
+    p.max_blocks = (uint32_t)append_max_blocks(b);
+    // Where the new tokens' blocks alone fill the card, a CTA takes all items of
+    // its block (one look-up, the next item's rows under way: 187 -> 145 us with q for
+    // 20,133 tokens of 8 heads, six CTAs an SM); a decode step's are spread, one each.
+    p.items = b.tokens / kKv8Block >= 2 * device_sm_count(device) ? 2 * c.kv_heads : 1;
+    p.groups = (uint32_t)((2 * c.kv_heads + p.items - 1) / p.items);
+    p.block_ctas = (uint32_t)(b.batch * p.max_blocks * p.groups);
+    p.magic_groups = kv8_magic(p.groups), p.magic_blocks = kv8_magic(p.max_blocks);
+    p.magic_page = kv8_magic((uint32_t)(c.page_size / kKv8Block));
     // a lane's D / 32 values as one vector
     const int size = act_bytes(a.dtype);
     const uintptr_t lane = (uintptr_t)(c.head_dim / 32 * size) - 1;

@@ -196,7 +196,7 @@ struct Kv8AppendArgs {
 // CTAs the append's launch needs at most.
 int64_t kv8_append_ctas(const vkq_kv8_cache &c, const vkq_kv8_batch &b, bool q);
 cudaError_t kv8_append(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_batch &b, const Kv8AppendArgs &a,
-                       cudaStream_t s);
+                       cudaStream_t s, int device);
 cudaError_t kv8_read(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_batch &b, const int *seq, const int *pos,
                      int64_t n, int dtype, void *k_out, void *v_out, cudaStream_t s);
 int kv8_read_status();
