@@ -19,8 +19,9 @@
 // within (0, 1], and out of the sum.  Both scales of 16 keys cost a thread two
 // multiplications a tile.
 //
-// 16-bit q: 256 rows, two halves of 128 in turn: while the scores of one half
-// are worked on, the products of the other run, and a K or V tile is converted
+// 16-bit q: 256 rows in two halves, each with a warpgroup, an issuing warp and
+// two score buffers of 64 keys: the scores of the next 64 keys are computed
+// while a warpgroup works on the ones before, and a K or V tile is converted
 // once for 256 rows.  e is rounded to 11 bits; the output stays in TMEM, and M
 // is raised (and the output rescaled) only when the maximum grew by more than
 // 2^8, which the operand's range allows.
@@ -51,13 +52,14 @@ static __device__ int g_kv8_prefill_status;
 constexpr int kPreThreads = 512;
 constexpr int kPreKeys = 128;                    // keys of a tile
 constexpr int kPreBlocks = kPreKeys / kKv8Block;  // and its scale blocks
+constexpr int kPreSub = 64;                       // keys whose scores a thread holds at once
 constexpr int kPreRing = 3;  // float16 tiles
 constexpr int kPreRaw = 3;   // tiles of codes
 constexpr uint32_t kPrePolls = 1u << 27;
 // registers a thread of warpgroups 0 and 1, of 2, of 3: at most 4 x 128 in all
 // (float32: warpgroup 1 holds a row's output)
 template <bool SPLIT> struct PreRegs {
-    static constexpr int score = SPLIT ? 176 : 160, convert = SPLIT ? 112 : 120, issue = SPLIT ? 48 : 64;
+    static constexpr int score = SPLIT ? 176 : 152, convert = SPLIT ? 72 : 96, issue = SPLIT ? 88 : 112;
     static_assert(2 * score + convert + issue <= 512, "more than the launch has");
     static_assert(score > 128 && convert < 128 && issue < 128, "setmaxnreg.inc grows, setmaxnreg.dec shrinks");
 };
@@ -222,7 +224,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
     // TMEM columns: the scores (and, over them, e) of half or parity 0 and 1, the outputs
     constexpr uint32_t kS = 0, kO = 256;
     extern __shared__ __align__(1024) uint8_t smem[];  // two q tiles, the rings
-    __shared__ __align__(8) uint64_t bars[2 * kPreRing + 2 * kPreRaw + 2 + 2 + 2 + 2 + 1];
+    __shared__ __align__(8) uint64_t bars[2 * kPreRing + 2 * kPreRaw + 4 + 4 + 2 + 2 + 1];
     __shared__ __align__(16) float scales[8][3][kPreBlocks];  // of key tile j & 7: ks, lv, 1 / vs
     __shared__ float alpha[4][128], lsum[128], msum[128], row_f[ROWS];
     __shared__ uint32_t tmem_slot;
@@ -265,23 +267,26 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
     const uint32_t base = (smem_u32addr(smem) + 1023u) & ~1023u;
     const uint32_t q_tile = base, ring = base + 2 * TILE, raw = ring + kPreRing * TILE;
     auto bar = [&](int i) { return smem_u32addr(&bars[i]); };
-    constexpr int FULL = 0, EMPTY = kPreRing, RF = 2 * kPreRing, RE = RF + kPreRaw, SF = RE + kPreRaw, PF = SF + 2, TF = PF + 2, TE = TF + 2, DR = TE + 2;
+    constexpr int FULL = 0, EMPTY = kPreRing, RF = 2 * kPreRing, RE = RF + kPreRaw, SF = RE + kPreRaw, PF = SF + 4, TF = PF + 4,
+                  TE = TF + 2, DR = TE + 2;
     if (tid == 0) {
         for (int i = 0; i < kPreRing; i++) {
             mbar_init(bar(FULL + i), 4);   // a lane of each converting warp
-            mbar_init(bar(EMPTY + i), 1);  // commit
+            mbar_init(bar(EMPTY + i), two ? 2 : 1);  // commits
         }
         for (int i = 0; i < kPreRaw; i++) {
             mbar_init(bar(RF + i), 1);  // the copies' bytes
             mbar_init(bar(RE + i), 4);  // a lane of each converting warp
         }
-        for (int i = 0; i < 2; i++) {
+        for (int i = 0; i < 4; i++) {  // of a half's two score buffers (SPLIT: of the two)
             mbar_init(bar(SF + i), 1);  // commit: scores
             mbar_init(bar(PF + i), 4);  // e is in TMEM
-            mbar_init(bar(TF + i), 1);  // commit: output (SPLIT: of one key tile)
-            mbar_init(bar(TE + i), 4);  // SPLIT: it has been read
         }
-        mbar_init(bar(DR), 1);
+        for (int i = 0; i < 2; i++) {
+            mbar_init(bar(TF + i), 1);              // commit: a half's output (SPLIT: of one key tile)
+            mbar_init(bar(TE + i), SPLIT ? 4 : 1);  // commit: a half's output up to a tile (SPLIT: it has been read)
+        }
+        mbar_init(bar(DR), two ? 2 : 1);  // commits: an issuer's last
         mbar_init_fence();
         abort_flag = 0;
         bad_flag = 0;
@@ -441,8 +446,9 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
                     if (uses) poll(bar(RF + i), (uses - 1) & 1u);
                 }
             __syncwarp();
-        } else if (warp == 12 && n > 0) {
-            constexpr uint32_t IQK = idesc_f16(kPreKeys, false), IPV = idesc_f16(D, true);
+        } else if ((warp == 12 || (warp == 14 && two)) && n > 0) {
+            // one issuer; with two halves one each (they share no scores or output)
+            constexpr uint32_t IQK = idesc_f16(SPLIT ? kPreKeys : kPreSub, false), IPV = idesc_f16(D, true);
             constexpr uint32_t HI = desc_hi(1024);  // eight rows of 128 bytes
             const uint32_t one = lane == 0;
             RingPos rp;
@@ -454,8 +460,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
                 rp.next(kPreRing);
             };
             // scores = q tile x K; K-major both: 16 values are 32 bytes into a 128-byte row
-            auto qk = [&](uint32_t d, uint32_t q, uint32_t slot, bool acc) {
-                const uint32_t da = desc_lo(q, 16u), db = desc_lo(ring + slot * TILE, 16u);
+            auto qk = [&](uint32_t d, uint32_t q, uint32_t k_tile, bool acc) {
+                const uint32_t da = desc_lo(q, 16u), db = desc_lo(k_tile, 16u);
 #pragma unroll
                 for (int k = 0; k < D / 16; k++) {
                     const uint32_t off = ((k >> 2) * HALF + (k & 3) * 32u) >> 4;
@@ -464,10 +470,10 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
             };
             // output = e x V; e: 16 keys are 8 of every 32 columns' first 16; V N-major: 16 keys
             // are 2048 bytes, the next 64 values HALF further
-            auto pv = [&](uint32_t d, uint32_t e, uint32_t slot, bool acc) {
-                const uint32_t db = desc_lo(ring + slot * TILE, HALF);
+            auto pv = [&](uint32_t d, uint32_t e, uint32_t v_tile, bool acc) {
+                const uint32_t db = desc_lo(v_tile, HALF);
 #pragma unroll
-                for (int k = 0; k < kPreKeys / 16; k++)
+                for (int k = 0; k < (SPLIT ? kPreKeys : kPreSub) / 16; k++)
                     umma_f16_ts(d, e + 32u * (k >> 1) + 8u * (k & 1), db + (k * 2048u >> 4), HI, IPV,
                                 (k > 0 || acc) ? 1u : 0u, one);
             };
@@ -478,8 +484,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
                     take(ks);
                     if (!ok) return;
                     const uint32_t d = tmem + kS + 128u * (j & 1);
-                    qk(d, q_tile, ks, false);
-                    qk(d, q_tile + TILE, ks, true);
+                    qk(d, q_tile, ring + ks * TILE, false);
+                    qk(d, q_tile + TILE, ring + ks * TILE, true);
                     commit(bar(SF + (j & 1)));
                     commit(bar(EMPTY + ks));
                 };
@@ -493,60 +499,43 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
                     if (!ok) break;
                     fence_after();
                     const uint32_t d = tmem + kO + 128u * b, e = tmem + kS + 128u * b;
-                    pv(d, e, vs, false);
-                    pv(d, e + 16u, vs, true);
+                    pv(d, e, ring + vs * TILE, false);
+                    pv(d, e + 16u, ring + vs * TILE, true);
                     commit(bar(TF + b));
                     commit(bar(EMPTY + vs));
                     if (j + 2 < n) scores(j + 2);
                 }
             } else {
+                const uint32_t hf = warp == 14, sc = tmem + kS + 128u * hf, o = tmem + kO + 128u * hf;
+                const uint32_t sf = SF + 2 * hf, pf = PF + 2 * hf;
+                // 64 keys of a tile are 8 KB of each half of its values
+                auto scores = [&](uint32_t b) {
+                    qk(sc + (uint32_t)kPreSub * b, q_tile + hf * TILE, ring + ks * TILE + b * (kPreSub * 128u), false);
+                    commit(bar(sf + b));
+                    if (b) commit(bar(EMPTY + ks));
+                };
                 take(ks);
-                if (ok) {
-                    qk(tmem + kS, q_tile, ks, false);
-                    commit(bar(SF));
-                    if (two) {
-                        qk(tmem + kS + 128u, q_tile + TILE, ks, false);
-                        commit(bar(SF + 1));
-                    }
-                    commit(bar(EMPTY + ks));
-                }
-                for (int j = 0; j < n && ok; j++) {
-                    const uint32_t ph = j & 1;
-                    const bool more = j + 1 < n;
-                    take(vs);
-                    if (ok) ok = wait_warp(bar(PF), ph);
+                if (ok) scores(0), scores(1);
+                for (int i = 0; i < 2 * n && ok; i++) {
+                    const uint32_t b = i & 1;
+                    if (b == 0) take(vs);
+                    ok = ok && wait_warp(bar(pf + b), (i >> 1) & 1);
                     if (!ok) break;
                     fence_after();
-                    pv(tmem + kO, tmem + kS, vs, j > 0);
-                    if (!two) commit(bar(EMPTY + vs));
-                    if (more) {
-                        take(ks);
+                    pv(o, sc + kPreSub * b, ring + vs * TILE + b * (kPreSub * 128u), i > 0);
+                    commit(bar(TE + hf));
+                    if (b) commit(bar(EMPTY + vs));
+                    if (i + 2 < 2 * n) {
+                        if (b == 0) take(ks);
                         if (!ok) break;
-                        qk(tmem + kS, q_tile, ks, false);
-                        commit(bar(SF));
-                        if (!two) commit(bar(EMPTY + ks));
-                    } else {
-                        commit(bar(TF));
-                    }
-                    if (two) {
-                        ok = wait_warp(bar(PF + 1), ph);
-                        if (!ok) break;
-                        fence_after();
-                        pv(tmem + kO + 128u, tmem + kS + 128u, vs, j > 0);
-                        commit(bar(EMPTY + vs));
-                        if (more) {
-                            qk(tmem + kS + 128u, q_tile + TILE, ks, false);
-                            commit(bar(SF + 1));
-                            commit(bar(EMPTY + ks));
-                        } else {
-                            commit(bar(TF + 1));
-                        }
+                        scores(b);
                     }
                 }
+                commit(bar(TF + hf));
             }
             // every product issued has finished before TMEM is given back
             commit(bar(DR));
-            wait_warp(bar(DR), 0);
+            if (warp == 12) wait_warp(bar(DR), 0);
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PreRegs<SPLIT>::score));
@@ -583,46 +572,53 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
             float m = -INFINITY, l = 0.f;
             const int warp_hi = __reduce_min_sync(0xffffffffu, see_hi), warp_lo = __reduce_max_sync(0xffffffffu, see_lo);
             bool ok = true;
-            for (int j = 0; j < n && ok; j++) {
-                const uint32_t b = SPLIT ? (j & 1) : wg;
-                const uint32_t ph = SPLIT ? (j >> 1) & 1 : j & 1;
-                ok = wait_warp(bar(SF + b), ph);
+            // a pass: 64 keys (SPLIT: a tile, its 64 scores at a time read twice)
+            constexpr int PARTS = SPLIT ? kPreKeys / kPreSub : 1;
+            const uint32_t hf = SPLIT ? 0 : wg;
+            for (int i = 0; i < (SPLIT ? n : 2 * n) && ok; i++) {
+                const uint32_t b = i & 1, ph = (i >> 1) & 1;
+                ok = wait_warp(bar(SF + 2 * hf + b), ph);
                 if (!ok) break;
                 fence_after();
-                const uint32_t sc = my + kS + 128u * b;
-                const int key = k_lo + j * kPreKeys;
-                const bool edge = key < warp_lo || key + kPreKeys > warp_hi;
-                const float *kss = scales[j & 7][0], *lvs = scales[j & 7][1], *inv = scales[j & 7][2];
-                // 32 scores (two blocks) at a time, twice: rolled loops, because the
-                // roles' code has to stay in the instruction cache together
-                uint32_t x[32];
-                auto scores = [&](int i) {
-                    tmem_ld32(x, sc + 32u * i);
-                    tmem_wait_ld(x);
+                const uint32_t sc = my + kS + (SPLIT ? 128u * b : 128u * hf + kPreSub * b);
+                const int j = SPLIT ? i : i >> 1;
+                const float *scl = scales[j & 7][0] + (SPLIT ? 0 : 4 * b);  // ks; lv and 1 / vs kPreBlocks further each
+                const int key = k_lo + i * (SPLIT ? kPreKeys : kPreSub);
+                const bool edge = key < warp_lo || key + (SPLIT ? kPreKeys : kPreSub) > warp_hi;
+                uint32_t x[2][32];
+                float kf[4], lv[4];
+                auto load = [&](int h) {
+                    tmem_ld32(x[0], sc + kPreSub * h);
+                    tmem_ld32(x[1], sc + kPreSub * h + 32u);
+                    const float4 a = *reinterpret_cast<const float4 *>(scl + 4 * h);
+                    const float4 c = *reinterpret_cast<const float4 *>(scl + kPreBlocks + 4 * h);
+                    // the factor above 0: -inf stays -inf
+                    kf[0] = fmaxf(a.x * rf, 1.4e-45f), kf[1] = fmaxf(a.y * rf, 1.4e-45f);
+                    kf[2] = fmaxf(a.z * rf, 1.4e-45f), kf[3] = fmaxf(a.w * rf, 1.4e-45f);
+                    lv[0] = c.x, lv[1] = c.y, lv[2] = c.z, lv[3] = c.w;
+                    tmem_wait_ld(x[0]);
+                    tmem_wait_ld(x[1]);
                     if (edge) {
-                        const int k0 = see_lo - key - 32 * i, k1 = see_hi - key - 32 * i;  // visible: [k0, k1)
+                        const int k0 = see_lo - key - kPreSub * h, k1 = see_hi - key - kPreSub * h;  // visible: [k0, k1)
 #pragma unroll
-                        for (int u = 0; u < 32; u++)
-                            if (u < k0 || u >= k1) x[u] = 0xff800000u;  // -inf
+                        for (int u = 0; u < kPreSub; u++)
+                            if (u < k0 || u >= k1) x[u / 32][u % 32] = 0xff800000u;  // -inf
                     }
                 };
-                // the tile's maximum of x + lv
+                // the maximum of x + lv
                 float mx = m;
 #pragma unroll 1
-                for (int i = 0; i < 4; i++) {
-                    scores(i);
+                for (int h = 0; h < PARTS; h++) {
+                    load(h);
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
+                    for (int q = 0; q < 4; q++) {
+                        const uint32_t *y = x[q / 2] + 16 * (q % 2);
                         float a[4];
 #pragma unroll
-                        for (int u = 0; u < 4; u++) {  // short chains: four at a time
-                            const uint32_t *y = x + 16 * h + 4 * u;
-                            a[u] = fmaxf(fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1])),
-                                         fmaxf(__uint_as_float(y[2]), __uint_as_float(y[3])));
-                        }
-                        const float top = fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3]));
-                        // the factor above 0: -inf stays -inf
-                        mx = fmaxf(mx, fmaf(top, fmaxf(kss[2 * i + h] * rf, 1.4e-45f), lvs[2 * i + h]));
+                        for (int u = 0; u < 4; u++)  // short chains: four at a time
+                            a[u] = fmaxf(fmaxf(__uint_as_float(y[4 * u]), __uint_as_float(y[4 * u + 1])),
+                                         fmaxf(__uint_as_float(y[4 * u + 2]), __uint_as_float(y[4 * u + 3])));
+                        mx = fmaxf(mx, fmaf(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])), kf[q], lv[q]));
                     }
                 }
                 float al = 1.f;
@@ -638,15 +634,18 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
                             al = ex2p(m - mx);
                             m = mx;
                         }
-                        if (j > 0) {
+                        if (i > 0) {
+                            ok = wait_warp(bar(TE + hf), (i - 1) & 1);  // the output of the keys before
+                            if (!ok) break;
+                            fence_after();
 #pragma unroll 1
-                            for (int i = 0; i < D / 8; i++) {
+                            for (int c = 0; c < D / 8; c++) {
                                 uint32_t o[8];
-                                tmem_ld8(o, my + kO + 128u * wg + 8u * i);
+                                tmem_ld8(o, my + kO + 128u * hf + 8u * c);
                                 tmem_wait_ld(o);
 #pragma unroll
                                 for (int u = 0; u < 8; u++) o[u] = __float_as_uint(__uint_as_float(o[u]) * al);
-                                tmem_st8(my + kO + 128u * wg + 8u * i, o);
+                                tmem_st8(my + kO + 128u * hf + 8u * c, o);
                             }
                         }
                     }
@@ -654,40 +653,45 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
                 l *= al;
                 const float off = m == -INFINITY ? 0.f : m - kUp;
 #pragma unroll 1
-                for (int i = 0; i < 4; i++) {
-                    scores(i);
-                    uint32_t hp[16];
+                for (int h = 0; h < PARTS; h++) {
+                    if (PARTS > 1) load(h);
+                    const float4 inv4 = *reinterpret_cast<const float4 *>(scl + 2 * kPreBlocks + 4 * h);
+                    const float inv[4] = {inv4.x, inv4.y, inv4.z, inv4.w};
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const float kf = fmaxf(kss[2 * i + h] * rf, 1.4e-45f), d = lvs[2 * i + h] - off;
-                        const float2 kf2 = make_float2(kf, kf), d2 = make_float2(d, d);
-                        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                    for (int q = 0; q < 2; q++) {  // 32 scores
+                        uint32_t hp[16];
 #pragma unroll
-                        for (int u = 0; u < 8; u++) {
-                            uint32_t *y = x + 16 * h + 2 * u;
-                            float2 e = f2fma(make_float2(__uint_as_float(y[0]), __uint_as_float(y[1])), kf2, d2);
-                            e.x = ex2p(e.x), e.y = ex2p(e.y);
-                            sum[u & 1] = f2add(sum[u & 1], e);
-                            y[0] = __float_as_uint(e.x), y[1] = __float_as_uint(e.y);
-                            hp[8 * h + u] = pack_half(e.x, e.y);
+                        for (int z = 0; z < 2; z++) {
+                            const float d = lv[2 * q + z] - off;
+                            const float2 kf2 = make_float2(kf[2 * q + z], kf[2 * q + z]), d2 = make_float2(d, d);
+                            float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+                            for (int u = 0; u < 8; u++) {
+                                uint32_t *y = x[q] + 16 * z + 2 * u;
+                                float2 e = f2fma(make_float2(__uint_as_float(y[0]), __uint_as_float(y[1])), kf2, d2);
+                                e.x = ex2p(e.x), e.y = ex2p(e.y);
+                                sum[u & 1] = f2add(sum[u & 1], e);
+                                y[0] = __float_as_uint(e.x), y[1] = __float_as_uint(e.y);
+                                hp[8 * z + u] = pack_half(e.x, e.y);
+                            }
+                            sum[0] = f2add(sum[0], sum[1]);
+                            l = fmaf(sum[0].x + sum[0].y, inv[2 * q + z], l);
                         }
-                        sum[0] = f2add(sum[0], sum[1]);
-                        l = fmaf(sum[0].x + sum[0].y, inv[2 * i + h], l);
-                    }
-                    // e as float16 over its scores: 16 columns (SPLIT: the low parts in the 16 after)
-                    tmem_st16(sc + 32u * i, hp);
-                    if constexpr (SPLIT) {
+                        // e as float16 over its scores: 16 columns (SPLIT: the low parts in the 16 after)
+                        tmem_st16(sc + kPreSub * h + 32u * q, hp);
+                        if constexpr (SPLIT) {
 #pragma unroll
-                        for (int u = 0; u < 16; u++) {
-                            const float2 back = unpack_half(hp[u]);
-                            hp[u] = pack_half(__uint_as_float(x[2 * u]) - back.x, __uint_as_float(x[2 * u + 1]) - back.y);
+                            for (int u = 0; u < 16; u++) {
+                                const float2 back = unpack_half(hp[u]);
+                                hp[u] = pack_half(__uint_as_float(x[q][2 * u]) - back.x, __uint_as_float(x[q][2 * u + 1]) - back.y);
+                            }
+                            tmem_st16(sc + kPreSub * h + 32u * q + 16u, hp);
                         }
-                        tmem_st16(sc + 32u * i + 16u, hp);
                     }
                 }
                 tmem_wait_st();
                 fence_before();
-                arrive(bar(PF + b));
+                arrive(bar(PF + 2 * hf + b));
             }
             if constexpr (SPLIT) {
                 lsum[t] = l, msum[t] = m;
@@ -764,13 +768,13 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
         last = active > 1 && atomicAdd(p.count + tile, 1u) == (unsigned)active - 1u;
     }
     __syncthreads();
-    if (!last) return;
+    if (!last || wg >= 2) return;  // warpgroups 2 and 3 have given registers away
     // the ranges' parts, in order
     __threadfence();
     if (tid == 0) p.count[tile] = 0;
     const float *part = p.part + tile * p.splits * ROWS * D, *stat = p.stat + tile * p.splits * ROWS * 2;
     const float nan = __int_as_float(0x7fc00000);
-    for (int i = tid; i < ROWS * D / 4; i += kPreThreads) {
+    for (int i = tid; i < ROWS * D / 4; i += 256) {
         const int r = i / (D / 4), d = i % (D / 4) * 4;
         if (r0 + r >= rows_all) break;
         float mx = -INFINITY;
