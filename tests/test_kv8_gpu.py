@@ -253,6 +253,81 @@ def test_strided_and_unaligned_rows(dtype):
         _attend(dtype, "int8", 6, 2, 64, 32, [300, 140], [150, 140], spare=spare)
 
 
+@pytest.fixture(params=[1 << 15, 1 << 18], ids=lambda n: f"bound{n}")
+def wide(request, monkeypatch):
+    """Tables whose bound on the lengths is large: many rows then take the 128-row
+    tiles, in several ranges of keys, whatever the lengths are."""
+    plain = _batch
+
+    def batch(table, lens, cu, slots=None, max_len=None):
+        pages = np.full((table.shape[0], request.param // 16), -1, np.int32)
+        pages[:, :table.shape[1]] = table
+        return plain(pages, lens, cu, slots, request.param)
+
+    monkeypatch.setitem(globals(), "_batch", batch)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("H,KVH,D", HEADS, ids=str)
+@pytest.mark.parametrize("page,lens,news,window", [
+    (64, [300, 129, 64], [7, 129, 0], 0), (64, [300, 129, 64], [7, 129, 1], 33), (32, [700], [257], 1),
+    (128, [513, 100], [512, 100], 100), (16, [3000, 1], [40, 1], 0)], ids=str)
+def test_many_rows_match_float64(wide, dtype, fmt, H, KVH, D, page, lens, news, window):
+    _attend(dtype, fmt, H, KVH, D, page, lens, news, window=window)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_many_rows_without_causal(wide, dtype):
+    _attend(dtype, "int8", 8, 2, 64, 32, [90], [90], causal=False)
+    _attend(dtype, "e4m3", 8, 2, 128, 64, [2500, 33], [40, 33], causal=False)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_many_rows_peaked_and_flat(wide, dtype):
+    test_peaked_and_flat_scores(dtype, 200)
+
+
+def test_many_rows_that_see_nothing(wide):
+    for dtype in ("f32", "bf16"):
+        got, _ = _attend(dtype, "e4m3", 8, 2, 128, 16, [3, 200], [150, 200])
+        assert (got[:147] == 0).all() and (got[147] != 0).any()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_many_rows_strided_and_unaligned(wide, dtype):
+    for spare in (1, 8, 64):
+        _attend(dtype, "int8", 6, 2, 64, 32, [300, 140], [150, 140], spare=spare)
+        _attend(dtype, "int8", 6, 2, 128, 32, [1300, 140], [150, 140], spare=spare)
+
+
+def test_many_rows_non_finite_query(wide):
+    test_non_finite_query_stays_in_its_row()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_many_rows_bad_pages(wide, dtype):
+    """A page out of bounds gives NaN for the rows that see it; other sequences are right."""
+    import torch
+    from vibrant_b200 import vkq
+    rng = np.random.default_rng(12)
+    pool = kh.Pool(200, 1, 16, 64, "int8", rng)
+    lens, news = [1300, 1300], 100
+    table = kh.table_for(rng, lens, 16, 200)
+    c = _cache(pool)
+    q = torch.randn(2 * news, 2, 64, device="cuda").to(getattr(torch, DT[dtype]))
+    cu = np.array([0, news, 2 * news])
+    for at, page in ((4, 200), (60, -1)):
+        wrong = table.copy()
+        wrong[1, at] = page
+        got = c.attend(0, _batch(wrong, lens, cu), q).float().cpu().numpy()
+        assert vkq.device_status(0) == vkq.ERR_INVALID_ARGUMENT
+        assert np.isnan(got[news:]).all()
+        out, bound, size = kh.attention(q.float().cpu().numpy()[:news], pool, table[:1], lens[:1], cu[:2], float(np.float32(0.125)))
+        assert float((np.abs(got[:news] - out) - kh.attention_tolerance(dtype, out, bound, size)).max()) <= 0
+    assert vkq.device_status(0) == vkq.OK
+
+
 def test_slots_and_output_strides():
     import torch
     from vibrant_b200 import kv8

@@ -14,11 +14,11 @@
 // order, so results do not depend on timing.
 //
 // The products run on m16n8k16 with float16 operands: codes are exact in
-// float16 (kv8_widen), and a decode step has at most 16 rows, where the 128-row tcgen05 tile would be
-// nearly empty.  Each lane's operand columns are chosen so that its 16-byte
+// float16 (kv8_widen), and a decode step has some 16 rows, which would leave a
+// 128-row tcgen05 tile nearly empty (many_rows has both sides measured).  Each lane's operand columns are chosen so that its 16-byte
 // loads from shared memory hold whole fragments: column k of a K step is
 // dimension 16 (c + 4 h) + 4 w + ..., column n of a V tile t is dimension
-// (D / 8) n + t; both are permutations that cancel.
+// (D / 8) n + t; the same order on both sides of a product, so it drops out.
 //
 // Precision.  float32 q and p are split, x = hi + lo with two float16 parts
 // (22 bits), one product each: with 8 rows the parts are rows r and r + 8 of
@@ -486,20 +486,30 @@ static const void *decode_fn(int D, bool e4m3, int rows) {
     return D == 64 ? decode_fn<T, 64, 8>(e4m3) : decode_fn<T, 128, 8>(e4m3);
 }
 
+// Keys that a tile of `rows` rows can see: all, or a window and the tile's own tokens.
+static int64_t seen_keys(const vkq_kv8_batch &b, int64_t rows, int64_t g, int causal, int64_t window) {
+    int64_t keys = b.max_len;
+    if (causal && window > 0) {
+        const int64_t w = window + (rows + g - 1) / g + kKv8Block;
+        if (w < keys) keys = w;
+    }
+    return keys < 1 ? 1 : keys;
+}
+
 static Kv8Plan decode_plan(const vkq_kv8_cache &c, const vkq_kv8_batch &b, int dtype, int64_t heads, int causal,
                               int64_t window, int sms) {
     Kv8Plan q{};
     const int64_t g = heads / c.kv_heads;
-    q.rows = dtype == VKQ_F32 || b.max_tokens * g <= 8 ? 8 : 16;
-    q.row_tiles = (int)((b.max_tokens * g + q.rows - 1) / q.rows);
+    const int64_t keys = seen_keys(b, 16, g, causal, window);
+    // 16-bit rows beyond eight: tiles of 16, which read the cache half as often,
+    // where they have a step for each CTA that the card holds, else tiles of 8.
+    // Measured in bfloat16, us in tiles of 8 / 16: 12 rows of 4,096 keys and 8 KV
+    // heads 16.2 / 19.2 (256 steps of a CTA), 30 rows of 32,768 57.9 / 45.2, 15
+    // rows of 32 contexts of 4,096 115 / 99.
+    const int64_t rows = b.max_tokens * g, steps = b.batch * c.kv_heads * ((rows + 15) / 16) * ((keys + 127) / 128);
+    q.rows = dtype == VKQ_F32 || rows <= 8 || steps < dec_ctas(16) * (int64_t)sms ? 8 : 16;
+    q.row_tiles = (int)((rows + q.rows - 1) / q.rows);
     q.tiles = b.batch * c.kv_heads * q.row_tiles;
-    // keys that a tile can see: all, or a window and the tile's own tokens
-    int64_t keys = b.max_len;
-    if (causal && window > 0) {
-        const int64_t w = window + (q.rows + g - 1) / g + kKv8Block;
-        if (w < keys) keys = w;
-    }
-    if (keys < 1) keys = 1;
     // Ranges: one sequence fills the card once (its ranges are alike, and are
     // joined by one CTA); several, of lengths that the host does not know, get
     // three times as many, so that the long ones spread.  At least one step a
@@ -522,15 +532,23 @@ static Kv8Plan decode_plan(const vkq_kv8_cache &c, const vkq_kv8_batch &b, int d
     return q;
 }
 
-// Rows of a sequence and KV head from which the 128-row tiles pay.
-static bool many_rows(const vkq_kv8_cache &c, const vkq_kv8_batch &b, int64_t heads) {
-    return b.max_tokens * (heads / c.kv_heads) > 64;
+// Whether the 128-row tiles of kv8_prefill.cu pay: more than 32 rows of a
+// sequence and KV head, and work for more than their 18 us of start and join.
+// Measured, us here / there, bfloat16 (float32): 32 contexts of 4,096 keys and 8
+// KV heads, 32 rows 166 / 185 (218 / 254), 64 rows 245 / 164 (378 / 229); one of
+// 32,768, 20 rows 48 / 59 (50 / 77), 40 rows 63 / 58 (73 / 74), 80 rows 92 / 56
+// (139 / 73); one of 2,048 and 2 KV heads, 64 rows 13 / 18 (14 / 18), 192 rows
+// (786,432 pairs of a row and a key) 22 / 21 (16 / 18), 512 rows 25 / 21 (26 / 20).
+static bool many_rows(const vkq_kv8_cache &c, const vkq_kv8_batch &b, int64_t heads, int causal, int64_t window) {
+    const int64_t g = heads / c.kv_heads, rows = b.max_tokens * g;
+    const double pairs = (double)(rows * c.kv_heads * b.batch) * (double)seen_keys(b, rows, g, causal, window);
+    return rows > 32 && pairs > (double)(1 << 19);
 }
 
 static Kv8Plan attention_plan(const vkq_kv8_cache &c, const vkq_kv8_batch &b, int dtype, int64_t heads, int causal,
                               int64_t window, int device) {
     const int sms = device_sm_count(device);
-    return many_rows(c, b, heads) ? kv8_prefill_plan(c, b, dtype, heads, causal, window, sms)
+    return many_rows(c, b, heads, causal, window) ? kv8_prefill_plan(c, b, dtype, heads, causal, window, sms)
                                   : decode_plan(c, b, dtype, heads, causal, window, sms);
 }
 
@@ -543,7 +561,7 @@ size_t kv8_attention_workspace(const vkq_kv8_cache &c, const vkq_kv8_batch &b, i
 cudaError_t kv8_attention(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_batch &b, const Kv8AttentionArgs &a,
                           cudaStream_t s, int device) {
     const Kv8Plan q = attention_plan(c, b, a.dtype, a.heads, a.causal, a.window, device);
-    if (many_rows(c, b, a.heads)) return kv8_prefill(c, layer, b, a, q, s);
+    if (many_rows(c, b, a.heads, a.causal, a.window)) return kv8_prefill(c, layer, b, a, q, s);
     DecodeParams p{};
     p.pool = kv8_pool(c, layer);
     p.batch = kv8_batch(b);

@@ -9,7 +9,7 @@
 //     shared memory, 16 tokens of a head (1 or 2 KB) a bulk copy, a ring of three;
 //   warpgroup 2 turns them into float16 K and V tiles (exact; 128-byte swizzle,
 //     one layout read K-major as K and MN-major as V), a ring of three;
-//   another warp of warpgroup 3 issues the products;
+//   other warps of warpgroup 3 (one a half of the rows) issue the products;
 //   warpgroups 0 and 1 work on the scores, a thread a row.
 // The block scales never touch the operands.  With x = f ks (q . ck) the
 // score of a key in units of log2 and lv = log2 vs,
@@ -32,8 +32,21 @@
 // works on the next scores.
 //
 // Row tiles go from the last (which sees most keys) to the first, so that the
-// longest start first.  Few tiles are split along the keys, and joined in
-// order by the CTA that finishes last.
+// longest start first.  Few tiles are split along the keys, and their parts
+// added in order by kv8_join_kernel.
+//
+// The copies and the conversion start while q is still on its way; an output
+// row goes out through shared memory, a whole line a store.  Loops that run
+// once a key tile stay together in the source, and are not unrolled further
+// than they need: with the start and the end of a block between them, their
+// instructions no longer stayed in the caches (4,096 tokens: 687 instead of
+// 620 us).
+//
+// Measured, 40 heads on 8 of D = 128: 4,096 new tokens of 8,192 in bfloat16 620
+// us, 830 TFLOP/s of q K and e V (1,843 of 12,288: 446 us, 960), in float32,
+// which takes four products for two, 1.10 ms; what bounds both is the hand-over
+// from loads to conversion to products to scores: without it the tensor pipe
+// would need 310 us, as it does twice that in float32.
 #include <atomic>
 #include <cmath>
 #include <cstdint>
@@ -75,7 +88,6 @@ struct PrefillParams {
     int causal, window;
     bool vec;
     float *part, *stat;
-    unsigned *count;
 };
 
 // Products issued by a whole warp, one lane of which (`one`) is the issuer: the
@@ -214,6 +226,20 @@ __device__ __forceinline__ uint32_t tile_off(int r, int pc) {
     return (uint32_t)((pc >> 3) * (kPreKeys * 128) + r * 128 + (((pc & 7) ^ (r & 7)) << 4));
 }
 
+// The keys that a tile of rows from r0 sees, and the ranges they are split into.
+struct PreKeySpan {
+    int lo, hi, active;
+};
+__device__ __forceinline__ PreKeySpan pre_keys(const PrefillParams &p, const Kv8Seq &s, int r0, int rows) {
+    const int pos0 = s.len - s.n, row_end = min(r0 + rows, s.n * p.g) - 1;
+    PreKeySpan k;
+    k.hi = p.causal ? max(pos0 + row_end / p.g + 1, 0) : s.len;
+    k.lo = 0;
+    if (p.window > 0) k.lo = max(pos0 + r0 / p.g - p.window + 1, 0) & ~(kKv8Block - 1);
+    k.active = max((k.hi - k.lo + p.chunk - 1) / p.chunk, 1);
+    return k;
+}
+
 template <typename T, int D, bool E4M3>
 __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const PrefillParams p) {
     constexpr bool SPLIT = sizeof(T) == 4;
@@ -230,7 +256,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
     __shared__ uint32_t tmem_slot;
     __shared__ volatile uint32_t abort_flag;
     __shared__ uint32_t bad_flag;
-    __shared__ bool last;
+    __shared__ int64_t q_row[ROWS], out_row[ROWS];  // where the rows are (out: -1 past the last)
     pdl_wait();
     pdl_launch_dependents();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = warp >> 2, t = tid & 127;
@@ -254,11 +280,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
     }
     if (r0 >= rows_all) return;
     const int pos0 = s.len - s.n;
-    const int row_end = min(r0 + ROWS, rows_all) - 1;
-    const int hi = p.causal ? max(pos0 + row_end / p.g + 1, 0) : s.len;
-    int lo = 0;
-    if (p.window > 0) lo = max(pos0 + r0 / p.g - p.window + 1, 0) & ~(kKv8Block - 1);
-    const int active = max((hi - lo + p.chunk - 1) / p.chunk, 1);
+    const PreKeySpan span = pre_keys(p, s, r0, ROWS);
+    const int lo = span.lo, hi = span.hi, active = span.active;
     if (split >= active) return;
     const int k_lo = lo + split * p.chunk, k_hi = min(hi, k_lo + p.chunk);
     const int n = k_hi > k_lo ? (k_hi - k_lo + kPreKeys - 1) / kPreKeys : 0;  // key tiles
@@ -291,49 +314,16 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
         abort_flag = 0;
         bad_flag = 0;
     }
-    if (warp == 12) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32addr(&tmem_slot)));
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-    }
-    // q: RT threads load a row, D / RT values each in one burst, scale it below
-    // 2^15 by a power of two and store its float16 tile (SPLIT: both parts)
-    {
-        constexpr int RT = kPreThreads / ROWS, PV = D / RT;
-        const int lr = tid / RT, c0 = (tid % RT) * PV, r = r0 + lr;
-        const bool there = r < rows_all;
-        const int i = there ? r / p.g : 0, h = kvh * p.g + (there ? r % p.g : 0);
-        float x[PV];
-        load_act<T, PV>(static_cast<const T *>(p.q) + (int64_t)(s.first + i) * p.qt + (int64_t)h * D + c0, x, p.vec);
-        float a = 0.f;
-#pragma unroll
-        for (int u = 0; u < PV; u++) a = fmaxf(a, fabsf(x[u]));
-#pragma unroll
-        for (int o = 1; o < RT; o <<= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-        const int e = min(max((int)(__float_as_uint(a) >> 23) - 127, -60), 127);
-        const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
-        if (tid % RT == 0) row_f[lr] = p.f * __uint_as_float((uint32_t)(e - 14 + 127) << 23);
-        const uint32_t dst = q_tile + (SPLIT ? 0u : (uint32_t)(lr / 128) * TILE);
-#pragma unroll
-        for (int c = 0; c < PV; c += 8) {
-            uint32_t b[4], b2[4];
-#pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const float x0 = x[c + 2 * u] * up, x1 = x[c + 2 * u + 1] * up;
-                b[u] = pack_half(x0, x1);
-                if constexpr (SPLIT) {
-                    const float2 back = unpack_half(b[u]);
-                    b2[u] = pack_half(x0 - back.x, x1 - back.y);
-                }
-            }
-            sts128(dst + tile_off(lr % 128, (c0 + c) / 8), b[0], b[1], b[2], b[3]);
-            if constexpr (SPLIT) sts128(dst + TILE + tile_off(lr % 128, (c0 + c) / 8), b2[0], b2[1], b2[2], b2[3]);
-        }
-        fence_async();
-    }
-    fence_before();
     __syncthreads();
-    fence_after();
-    const uint32_t tmem = tmem_slot;
+    uint32_t tmem = 0;
+    // The copies and the conversion start at once; those who need q and TMEM
+    // (warpgroups 0 and 1, the issuing warps) meet here.
+    auto meet = [&]() {
+        fence_before();
+        asm volatile("bar.sync 2, 320;" ::: "memory");
+        fence_after();
+        tmem = tmem_slot;
+    };
 
     // for whole warps: one lane polls
     auto wait_warp = [&](uint32_t b, uint32_t parity) -> bool {
@@ -347,6 +337,63 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
     };
 
     const int64_t tile = ((int64_t)seq * p.pool.kv_heads + kvh) * p.row_tiles + rt;
+    const float nan = __int_as_float(0x7fc00000);
+    const int row = SPLIT ? t : 128 * wg + t;  // of warpgroups 0 and 1
+    int row_token = 0;
+    bool there = false;
+    float m = -INFINITY, l = 0.f;
+    if (wg < 2) {
+        there = r0 + row < rows_all;
+        row_token = there ? (r0 + row) / p.g : 0;
+        const int row_head = kvh * p.g + (there ? r0 + row - row_token * p.g : 0);
+        if (!SPLIT || wg == 0) {
+            q_row[row] = (int64_t)(s.first + row_token) * p.qt + (int64_t)row_head * D;
+            out_row[row] = there ? (int64_t)(s.first + row_token) * p.ot + (int64_t)row_head * D : -1;
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        // q: consecutive lanes load a row's consecutive eight values, scale them
+        // by the row's power of two, below 2^15, and store the float16 tile
+        // (SPLIT: both parts)
+        {
+            constexpr int PR = D / 8, PIECES = ROWS * PR / 256, QB = PIECES < 4 * (int)sizeof(float) / (int)sizeof(T) ? PIECES : 4 * (int)sizeof(float) / (int)sizeof(T);
+#pragma unroll 1
+            for (int b0 = 0; b0 < PIECES; b0 += QB) {
+                float x[QB][8];
+#pragma unroll
+                for (int b = 0; b < QB; b++) {
+                    const int lr = ((b0 + b) * 256 + tid) / PR;
+                    load_act<T, 8>(static_cast<const T *>(p.q) + q_row[lr] + tid % PR * 8, x[b], p.vec);
+                }
+#pragma unroll
+                for (int b = 0; b < QB; b++) {
+                    const int lr = ((b0 + b) * 256 + tid) / PR;
+                    float a = 0.f;
+#pragma unroll
+                    for (int u = 0; u < 8; u++) a = fmaxf(a, fabsf(x[b][u]));
+#pragma unroll
+                    for (int o = 1; o < PR; o <<= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+                    const int e = min(max((int)(__float_as_uint(a) >> 23) - 127, -60), 127);
+                    const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
+                    if (tid % PR == 0) row_f[lr] = p.f * __uint_as_float((uint32_t)(e - 14 + 127) << 23);
+                    const uint32_t dst = q_tile + (SPLIT ? 0u : (uint32_t)(lr / 128) * TILE) + tile_off(lr % 128, tid % PR);
+                    uint32_t w[4], w2[4];
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        const float x0 = x[b][2 * u] * up, x1 = x[b][2 * u + 1] * up;
+                        w[u] = pack_half(x0, x1);
+                        if constexpr (SPLIT) {
+                            const float2 back = unpack_half(w[u]);
+                            w2[u] = pack_half(x0 - back.x, x1 - back.y);
+                        }
+                    }
+                    sts128(dst, w[0], w[1], w[2], w[3]);
+                    if constexpr (SPLIT) sts128(dst + TILE, w2[0], w2[1], w2[2], w2[3]);
+                }
+            }
+            fence_async();
+            meet();
+        }
+    }
     // The tiles in the order in which the products take them: K0, then V(j),
     // K(j + 1) (SPLIT: K(j + 1), V(j): the scores of a tile are asked for before
     // the output of the one before).
@@ -361,6 +408,54 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
         b.k_done = a.k_done + !b.is_v, b.v_done = a.v_done + b.is_v;
         return b;
     };
+            // Eight values from dimension c.  A row of out goes through shared memory
+            // (the half's q tile, done with by then), in pieces of 16 bytes swizzled
+            // by the row, so that a warp stores whole lines: rows stored by their
+            // threads took 8,000 clocks a block.
+            // (What they need is worked out here: kept over the loop it cost registers
+            // there, and 3% of a long prompt's time.)
+            constexpr int PC = D * (int)sizeof(T) / 16, N = 16 / (int)sizeof(T);
+            auto stage = [&]() { return smem + (q_tile - smem_u32addr(smem)) + (SPLIT ? 0u : wg * TILE); };
+            auto put = [&](int c, float (&v)[8], float inv) {
+                if (active > 1) {  // this range's part, rows fastest
+                    float4 *d = reinterpret_cast<float4 *>(p.part + (tile * p.splits + split) * ROWS * D) + c / 4 * ROWS + row;
+                    d[0] = make_float4(v[0], v[1], v[2], v[3]);
+                    d[ROWS] = make_float4(v[4], v[5], v[6], v[7]);
+                } else {
+    #pragma unroll
+                    for (int u = 0; u < 8; u++) v[u] *= inv;
+    #pragma unroll
+                    for (int z = 0; z < 8; z += N) {
+                        float piece[N];
+    #pragma unroll
+                        for (int u = 0; u < N; u++) piece[u] = v[z + u];
+                        store_act<T, N>(reinterpret_cast<T *>(stage() + t * (16 * PC) + ((((c + z) / N) ^ (t & 7)) << 4)), piece, true);
+                    }
+                }
+            };
+            auto put_stat = [&](float m, float l) {
+                if (active > 1) reinterpret_cast<float2 *>(p.stat + (tile * p.splits + split) * ROWS * 2)[row] = make_float2(m, l);
+            };
+            auto put_end = [&]() {
+                if (active > 1) return;
+                __syncwarp();
+    #pragma unroll 4
+                for (int i = lane; i < 32 * PC; i += 32) {
+                    const int from = 32 * (warp & 3) + i / PC, pc = i % PC;
+                    const int64_t o = out_row[SPLIT ? from : 128 * wg + from];
+                    if (o < 0) continue;
+                    const uint4 v = *reinterpret_cast<const uint4 *>(stage() + from * (16 * PC) + ((pc ^ (from & 7)) << 4));
+                    T *const dst = static_cast<T *>(p.out) + o + pc * N;
+                    if (p.vec) {
+                        *reinterpret_cast<uint4 *>(dst) = v;
+                    } else {
+                        alignas(16) T e[N];
+                        *reinterpret_cast<uint4 *>(e) = v;
+    #pragma unroll
+                        for (int u = 0; u < N; u++) dst[u] = e[u];
+                    }
+                }
+            };
     if (wg == 2) {
         // ---- codes to float16 tiles ----
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PreRegs<SPLIT>::convert));
@@ -379,7 +474,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
             if (rp.uses >= (uint32_t)kPreRing && !wait_warp(bar(EMPTY + rp.idx), rp.phase ^ 1u)) break;
             const uint32_t dst = ring + rp.idx * TILE, src = raw + rr.idx * (TILE / 2) + (uint32_t)(row0 * D + ch * 16);
             const int left = k_hi - (k_lo + item.j * kPreKeys) - row0;  // rows past the range are zeros
-#pragma unroll 2
+#pragma unroll 1
             for (int k = 0; k < PER; k++) {
                 uint4 c = lds128(src + (uint32_t)k * (RSTEP * D));
                 if (k * RSTEP >= left) c = make_uint4(0, 0, 0, 0);
@@ -398,6 +493,11 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
     } else if (wg == 3) {
         // ---- the products ----
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PreRegs<SPLIT>::issue));
+        if (warp == 12) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32addr(&tmem_slot)));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        }
+        if (warp == 12 || warp == 14) meet();
         if (warp == 13 && n > 0) {
             // the tiles' pages: lane b takes block b
             const uint32_t per_page = (uint32_t)(p.pool.page / kKv8Block), magic = 0xffffffffu / per_page + 1u;
@@ -540,36 +640,12 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PreRegs<SPLIT>::score));
         const uint32_t my = tmem + ((uint32_t)(32 * (warp & 3)) << 16);  // the warp's lanes
-        // the rows' outputs: `part` and `stat` of this range, or out
-        float *part = p.part + (tile * p.splits + split) * ROWS * D;
-        float *stat = p.stat + (tile * p.splits + split) * ROWS * 2;
-        const int row = SPLIT ? t : 128 * wg + t;
-        T *out_row = nullptr;
-        if (r0 + row < rows_all)
-            out_row = static_cast<T *>(p.out) + (int64_t)(s.first + (r0 + row) / p.g) * p.ot +
-                      (int64_t)(kvh * p.g + (r0 + row) % p.g) * D;
-        auto put = [&](int c, float (&v)[8], float l) {  // eight values from dimension c
-            if (!out_row) return;
-            if (active > 1) {
-                float4 *d = reinterpret_cast<float4 *>(part + (int64_t)row * D + c);
-                d[0] = make_float4(v[0], v[1], v[2], v[3]);
-                d[1] = make_float4(v[4], v[5], v[6], v[7]);
-            } else {
-                const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-                for (int u = 0; u < 8; u++) v[u] *= inv;
-                store_act<T, 8>(out_row + c, v, p.vec);
-            }
-        };
-        const float nan = __int_as_float(0x7fc00000);
         if (wg == 0 || (!SPLIT && two)) {
             // ---- scores to e ----
-            const bool there = r0 + row < rows_all;
-            const int ps = pos0 + (there ? (r0 + row) / p.g : 0);  // the row's position; it sees [see_lo, see_hi)
+            const int ps = pos0 + row_token;  // the row's position; it sees [see_lo, see_hi)
             const int see_hi = !there ? 0 : min(p.causal ? ps + 1 : s.len, k_hi);
             const int see_lo = p.window > 0 ? ps - p.window + 1 : 0;
             const float rf = row_f[row];
-            float m = -INFINITY, l = 0.f;
             const int warp_hi = __reduce_min_sync(0xffffffffu, see_hi), warp_lo = __reduce_max_sync(0xffffffffu, see_lo);
             bool ok = true;
             // a pass: 64 keys (SPLIT: a tile, its 64 scores at a time read twice)
@@ -696,29 +772,6 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
             if constexpr (SPLIT) {
                 lsum[t] = l, msum[t] = m;
                 asm volatile("bar.sync 1, 256;" ::: "memory");
-            } else {
-                const bool got = n > 0 && wait_warp(bar(TF + wg), 0);
-                fence_after();
-                if (bad_flag || abort_flag) l = nan;
-                if (active > 1 && out_row) stat[2 * row] = m, stat[2 * row + 1] = l;
-#pragma unroll
-                for (int i = 0; i < D / 32; i++) {
-                    uint32_t o[32];
-                    if (got) {
-                        tmem_ld32(o, my + kO + 128u * wg + 32u * i);
-                        tmem_wait_ld(o);
-                    } else {
-#pragma unroll
-                        for (int u = 0; u < 32; u++) o[u] = 0;
-                    }
-#pragma unroll
-                    for (int c = 0; c < 32; c += 8) {
-                        float v[8];
-#pragma unroll
-                        for (int u = 0; u < 8; u++) v[u] = __uint_as_float(o[c + u]);
-                        put(32 * i + c, v, l);
-                    }
-                }
             }
         } else if constexpr (SPLIT) {
             // ---- the key tiles' outputs, added in float32 ----
@@ -743,20 +796,49 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
             }
             // l and M are warpgroup 0's: its last e came before the last output
             asm volatile("bar.sync 1, 256;" ::: "memory");
-            float l = lsum[t];
+            l = lsum[t];
             if (bad_flag || abort_flag) l = nan;
-            if (active > 1 && out_row) stat[2 * row] = msum[t], stat[2 * row + 1] = l;
+            put_stat(msum[t], l);
+            const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
             for (int c = 0; c < D; c += 8) {
                 float v[8];
 #pragma unroll
                 for (int u = 0; u < 8; u++) v[u] = acc[c + u];
-                put(c, v, l);
+                put(c, v, inv);
             }
+            put_end();
+        }
+    }
+    if constexpr (!SPLIT) {
+        if (wg == 0 || (wg == 1 && two)) {
+            const bool got = n > 0 && wait_warp(bar(TF + wg), 0);
+            fence_after();
+            if (bad_flag || abort_flag) l = nan;
+            put_stat(m, l);
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll 1
+            for (int i = 0; i < D / 32; i++) {
+                uint32_t o[32];
+                if (got) {
+                    tmem_ld32(o, tmem + ((uint32_t)(32 * (warp & 3)) << 16) + kO + 128u * wg + 32u * i);
+                    tmem_wait_ld(o);
+                } else {
+#pragma unroll
+                    for (int u = 0; u < 32; u++) o[u] = 0;
+                }
+#pragma unroll
+                for (int c = 0; c < 32; c += 8) {
+                    float v[8];
+#pragma unroll
+                    for (int u = 0; u < 8; u++) v[u] = __uint_as_float(o[c + u]);
+                    put(32 * i + c, v, inv);
+                }
+            }
+            put_end();
         }
     }
     fence_before();
-    if (active > 1) __threadfence();
     __syncthreads();
     if (warp == 12) {
         fence_after();
@@ -765,35 +847,61 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
     if (tid == 0) {
         if (bad_flag) atomicExch(&g_kv8_prefill_status, VKQ_ERR_INVALID_ARGUMENT);
         if (abort_flag) atomicExch(&g_kv8_prefill_status, kStatusTimeout);
-        last = active > 1 && atomicAdd(p.count + tile, 1u) == (unsigned)active - 1u;
     }
-    __syncthreads();
-    if (!last || wg >= 2) return;  // warpgroups 2 and 3 have given registers away
-    // the ranges' parts, in order
-    __threadfence();
-    if (tid == 0) p.count[tile] = 0;
-    const float *part = p.part + tile * p.splits * ROWS * D, *stat = p.stat + tile * p.splits * ROWS * 2;
-    const float nan = __int_as_float(0x7fc00000);
-    for (int i = tid; i < ROWS * D / 4; i += 256) {
-        const int r = i / (D / 4), d = i % (D / 4) * 4;
-        if (r0 + r >= rows_all) break;
-        float mx = -INFINITY;
-        for (int w = 0; w < active; w++) mx = fmaxf(mx, __ldcg(stat + (w * ROWS + r) * 2));
-        float sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int w = 0; w < active; w++) {
-            const float2 ms = __ldcg(reinterpret_cast<const float2 *>(stat + (w * ROWS + r) * 2));
-            const float4 v = __ldcg(reinterpret_cast<const float4 *>(part + ((int64_t)w * ROWS + r) * D + d));
-            const float k = ms.x == -INFINITY ? (ms.y == ms.y ? 0.f : nan) : ex2p(ms.x - mx);
-            sum += k * ms.y;
-            acc[0] += k * v.x, acc[1] += k * v.y, acc[2] += k * v.z, acc[3] += k * v.w;
-        }
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+}
+
+// The outputs of tiles that were split along the keys, the ranges' parts added
+// in their order.  A block takes 32 rows, a warp an eighth of their values, a
+// lane a row.  A launch of its own, because the last block of a tile to finish
+// reads its ranges at one SM's bandwidth only: 12 us for 6 ranges of 256 rows.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) kv8_join_kernel(const PrefillParams p) {
+    constexpr int ROWS = sizeof(T) == 4 ? 128 : 256, TD = D / 8, AT = 4;
+    pdl_wait();
+    pdl_launch_dependents();
+    const int lane = threadIdx.x & 31, d0 = (threadIdx.x >> 5) * TD;
+    const int64_t tile = blockIdx.x / (ROWS / 32);
+    const int rt = (int)(tile % p.row_tiles), kvh = (int)(tile / p.row_tiles % p.pool.kv_heads);
+    const Kv8Seq s = kv8_seq(p.batch, p.pool.page, (int)(tile / p.row_tiles / p.pool.kv_heads));
+    const int tr = (int)(blockIdx.x % (ROWS / 32)) * 32 + lane, r = rt * ROWS + tr;
+    if (!s.ok || r >= s.n * p.g) return;
+    const int active = pre_keys(p, s, rt * ROWS, ROWS).active;
+    if (active < 2) return;
+    const float4 *part = reinterpret_cast<const float4 *>(p.part + tile * p.splits * ROWS * D) + d0 / 4 * ROWS + tr;
+    const float2 *stat = reinterpret_cast<const float2 *>(p.stat + tile * p.splits * ROWS * 2) + tr;
+    float mx = -INFINITY, sum = 0.f, acc[TD];
+#pragma unroll 8
+    for (int w = 0; w < active; w++) mx = fmaxf(mx, __ldcg(stat + w * ROWS).x);
 #pragma unroll
-        for (int z = 0; z < 4; z++) acc[z] *= inv;
-        store_act<T, 4>(static_cast<T *>(p.out) + (int64_t)(s.first + (r0 + r) / p.g) * p.ot +
-                            (int64_t)(kvh * p.g + (r0 + r) % p.g) * D + d,
-                        acc, p.vec);
+    for (int u = 0; u < TD; u++) acc[u] = 0.f;
+    for (int w = 0; w < active; w += AT) {
+        float4 v[AT][TD / 4];
+        float2 ms[AT];
+#pragma unroll
+        for (int z = 0; z < AT; z++) {
+            const bool is = w + z < active;
+            ms[z] = is ? __ldcg(stat + (w + z) * ROWS) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int u = 0; u < TD / 4; u++)
+                v[z][u] = is ? __ldcg(part + (int64_t)(w + z) * (ROWS * D / 4) + u * ROWS) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int z = 0; z < AT; z++) {
+            // a range without a visible key weighs nothing; a NaN sum spreads
+            const float k = ms[z].x == -INFINITY ? (ms[z].y == ms[z].y ? 0.f : ms[z].y) : ex2p(ms[z].x - mx);
+            sum = fmaf(k, ms[z].y, sum);
+#pragma unroll
+            for (int u = 0; u < TD / 4; u++) {
+                acc[4 * u] = fmaf(k, v[z][u].x, acc[4 * u]), acc[4 * u + 1] = fmaf(k, v[z][u].y, acc[4 * u + 1]);
+                acc[4 * u + 2] = fmaf(k, v[z][u].z, acc[4 * u + 2]), acc[4 * u + 3] = fmaf(k, v[z][u].w, acc[4 * u + 3]);
+            }
+        }
     }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int u = 0; u < TD; u++) acc[u] *= inv;
+    store_act<T, TD>(static_cast<T *>(p.out) + (int64_t)(s.first + r / p.g) * p.ot + (int64_t)(kvh * p.g + r % p.g) * D + d0, acc,
+                     p.vec);
 }
 
 template <typename T, int D>
@@ -803,6 +911,11 @@ static const void *prefill_fn(bool e4m3) {
 template <typename T>
 static const void *prefill_fn(int D, bool e4m3) {
     return D == 64 ? prefill_fn<T, 64>(e4m3) : prefill_fn<T, 128>(e4m3);
+}
+
+template <typename T>
+static const void *join_fn(int D) {
+    return D == 64 ? (const void *)kv8_join_kernel<T, 64> : (const void *)kv8_join_kernel<T, 128>;
 }
 
 Kv8Plan kv8_prefill_plan(const vkq_kv8_cache &c, const vkq_kv8_batch &b, int dtype, int64_t heads, int causal,
@@ -818,16 +931,27 @@ Kv8Plan kv8_prefill_plan(const vkq_kv8_cache &c, const vkq_kv8_batch &b, int dty
         if (w < keys) keys = w;
     }
     if (keys < 1) keys = 1;
-    // one CTA an SM: ranges of at least four key tiles until there are two waves
-    int64_t splits = 2 * (int64_t)sms / q.tiles;
-    const int64_t most = (keys + 4 * kPreKeys - 1) / (4 * kPreKeys);
-    if (splits > most) splits = most;
-    if (splits > 64) splits = 64;
-    if (splits < 1 || q.tiles > kHeadCounters) splits = 1;
-    int64_t chunk = (keys + splits - 1) / splits;
-    chunk = (chunk + kPreKeys - 1) / kPreKeys * kPreKeys;
-    q.chunk = (int)chunk;
-    q.splits = (int)((keys + chunk - 1) / chunk);
+    // Ranges: what is cheapest in units of a key tile's time (2.3 to 2.8 us), a
+    // CTA an SM.  A CTA costs its key tiles (a causal tile sees all but half of
+    // the new tokens on average) and kStart for its start and end; ranges cost
+    // the join's launch and their parts' bytes.  Measured, 8 KV heads, bfloat16:
+    // 512 rows of 65,536 keys (24 tiles) 1,377 us in one range, 362 in 4, 251 in
+    // 6 (chosen), 347 in 8; 2,560 rows of 8,192 keys (80 tiles) 183, 151 in 3
+    // (chosen), 236 in 16; 5,120 rows of 1,024 keys (160) 35 (chosen), 54 in 2.
+    constexpr double kStart = 3., kJoin = 1.5, kPart = 0.019 / (256 * 128);
+    const int64_t most = (keys + kPreKeys - 1) / kPreKeys;
+    double seen = causal ? (double)keys - 0.5 * (double)(b.max_tokens < keys ? b.max_tokens : keys) : (double)keys;
+    if (causal && window > 0) seen = (double)keys;
+    int64_t best = most;  // a range's key tiles
+    double least = 0.;
+    for (int64_t n = 1; n <= 64 && n <= most; n++) {
+        const int64_t tiles = (most + n - 1) / n, ranges = (most + tiles - 1) / tiles, ctas = q.tiles * ranges;
+        double cost = (double)((ctas + sms - 1) / sms) * ((double)tiles * seen / (double)keys + kStart);
+        if (ranges > 1) cost += kJoin + (double)(ctas * q.rows * c.head_dim) * kPart;
+        if (n == 1 || cost < least) best = tiles, least = cost;
+    }
+    q.chunk = (int)(best * kPreKeys);
+    q.splits = (int)((most + best - 1) / best);
     if (q.splits > 1) {
         q.part_floats = (size_t)(q.tiles * q.splits * q.rows * c.head_dim);
         q.stat_floats = (size_t)(q.tiles * q.splits * q.rows * 2);
@@ -847,7 +971,6 @@ cudaError_t kv8_prefill(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_bat
     p.causal = a.causal, p.window = a.causal ? (int)a.window : 0;
     const int size = act_bytes(a.dtype);
     p.vec = (((uintptr_t)a.q | (uintptr_t)a.out | (uintptr_t)(a.q_token * size) | (uintptr_t)(a.out_token * size)) & 15u) == 0;
-    p.count = static_cast<unsigned *>(a.workspace);
     p.part = reinterpret_cast<float *>(static_cast<char *>(a.workspace) + kWorkspaceCounterHead);
     p.stat = p.part + q.part_floats;
     const void *fn = a.dtype == VKQ_F32   ? prefill_fn<float>(c.head_dim, p.pool.e4m3)
@@ -878,7 +1001,15 @@ cudaError_t kv8_prefill(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_bat
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     void *args[] = {(void *)&p};
-    return cudaLaunchKernelExC(&cfg, fn, args);
+    e = cudaLaunchKernelExC(&cfg, fn, args);
+    if (e != cudaSuccess || q.splits == 1) return e;
+    cfg.gridDim = dim3((unsigned)(q.tiles * (q.rows / 32)));
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = 0;
+    const void *join = a.dtype == VKQ_F32   ? join_fn<float>(c.head_dim)
+                       : a.dtype == VKQ_F16 ? join_fn<__half>(c.head_dim)
+                                            : join_fn<__nv_bfloat16>(c.head_dim);
+    return cudaLaunchKernelExC(&cfg, join, args);
 }
 
 int kv8_prefill_read_status() {
