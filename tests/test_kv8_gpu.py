@@ -340,6 +340,31 @@ def test_many_rows_bad_pages(wide, dtype):
     assert vkq.device_status(0) == vkq.OK
 
 
+def test_many_rows_bad_offsets(wide):
+    """Token offsets and lengths out of bounds: reported, NaN where the rows are known."""
+    import torch
+    from vibrant_b200 import vkq
+    rng = np.random.default_rng(13)
+    pool = kh.Pool(40, 1, 16, 64, "int8", rng)
+    lens = [130, 130]
+    table = kh.table_for(rng, lens, 16, 40)
+    c = _cache(pool)
+    q = torch.randn(200, 2, 64, device="cuda")
+    want = c.attend(0, _batch(table, lens, [0, 100, 200]), q)
+    assert vkq.device_status(0) == vkq.OK
+    for cu in ([0, 100, 205], [0, 100, 90], [-1, 100, 200]):
+        b = _batch(table, lens, [0, 100, 200])
+        b.tensors[3].copy_(torch.tensor(cu, dtype=torch.int32))
+        got = c.attend(0, b, q)
+        assert vkq.device_status(0) == vkq.ERR_INVALID_ARGUMENT
+        good = slice(0, 100) if cu[0] == 0 else slice(100, 200)
+        assert torch.equal(got[good], want[good])
+    got = c.attend(0, _batch(table, [-1, 130], [0, 100, 200]), q)
+    assert vkq.device_status(0) == vkq.ERR_INVALID_ARGUMENT
+    assert bool(torch.isnan(got[:100]).all()) and torch.equal(got[100:], want[100:])
+    assert vkq.device_status(0) == vkq.OK
+
+
 def test_slots_and_output_strides():
     import torch
     from vibrant_b200 import kv8

@@ -18,9 +18,8 @@
 // atomics and the result does not depend on the order of anything.  Latency
 // bounds a decode step (48 sequences: 10 us with the read-back), the
 // instructions a value a prompt (20,133 tokens in bfloat16, 8 KV heads and q's
-// 40: 145 us); q's rotation rides in
-// the same launch (CTAs past the blocks', a few tokens each),
-// which saves a launch a layer.
+// 40: 145 us); q's rotation rides in the same launch (CTAs past the blocks', a
+// few tokens each), which saves a launch a layer.
 #include <cstdint>
 
 #include "../../include/vkq.h"

@@ -31,8 +31,8 @@
 // from zero, and warpgroup 1 adds it to float32 registers while warpgroup 0
 // works on the next scores.
 //
-// Row tiles go from the last (which sees most keys) to the first, so that the
-// longest start first.  Few tiles are split along the keys, and their parts
+// Row tiles go from each sequence's last (which sees most keys) to its first, so
+// that the longest start first.  Few tiles are split along the keys, and their parts
 // added in order by kv8_join_kernel.
 //
 // The copies and the conversion start while q is still on its way; an output
@@ -263,13 +263,15 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
     // block = ((reversed row tile, range), sequence, KV head), the last fastest
     const int kvh = (int)(blockIdx.x % p.pool.kv_heads), x0 = (int)(blockIdx.x / p.pool.kv_heads);
     const int seq = x0 % (int)p.batch.batch, x1 = x0 / (int)p.batch.batch;
-    const int rt = p.row_tiles - 1 - x1 / p.splits, split = x1 % p.splits;
+    const int split = x1 % p.splits;
     const Kv8Seq s = kv8_seq(p.batch, p.pool.page, seq);
     const int rows_all = s.n * p.g;
+    const int rt = (rows_all + ROWS - 1) / ROWS - 1 - x1 / p.splits;  // from the sequence's own last
     const int r0 = rt * ROWS;
     if (!s.ok) {
         if (split > 0) return;
         if (tid == 0) atomicExch(&g_kv8_prefill_status, VKQ_ERR_INVALID_ARGUMENT);
+        if (rt < 0) return;
         for (int64_t i = tid; i < (int64_t)ROWS * D; i += kPreThreads) {
             const int r = r0 + (int)(i / D);
             if (r < rows_all)
@@ -278,7 +280,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
         }
         return;
     }
-    if (r0 >= rows_all) return;
+    if (rt < 0) return;
     const int pos0 = s.len - s.n;
     const PreKeySpan span = pre_keys(p, s, r0, ROWS);
     const int lo = span.lo, hi = span.hi, active = span.active;
@@ -355,7 +357,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
         // by the row's power of two, below 2^15, and store the float16 tile
         // (SPLIT: both parts)
         {
-            constexpr int PR = D / 8, PIECES = ROWS * PR / 256, QB = PIECES < 4 * (int)sizeof(float) / (int)sizeof(T) ? PIECES : 4 * (int)sizeof(float) / (int)sizeof(T);
+            constexpr int PR = D / 8, PIECES = ROWS * PR / 256, QB = SPLIT || PIECES < 8 ? 4 : 8;
 #pragma unroll 1
             for (int b0 = 0; b0 < PIECES; b0 += QB) {
                 float x[QB][8];
@@ -418,7 +420,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
             auto stage = [&]() { return smem + (q_tile - smem_u32addr(smem)) + (SPLIT ? 0u : wg * TILE); };
             auto put = [&](int c, float (&v)[8], float inv) {
                 if (active > 1) {  // this range's part, rows fastest
-                    float4 *d = reinterpret_cast<float4 *>(p.part + (tile * p.splits + split) * ROWS * D) + c / 4 * ROWS + row;
+                    float *const part = p.part + (tile * p.splits + split) * ROWS * D;
+                float4 *d = reinterpret_cast<float4 *>(part) + c / 4 * ROWS + row;
                     d[0] = make_float4(v[0], v[1], v[2], v[3]);
                     d[ROWS] = make_float4(v[4], v[5], v[6], v[7]);
                 } else {
