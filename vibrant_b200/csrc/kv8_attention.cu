@@ -517,19 +517,36 @@ static Kv8Plan decode_plan(const vkq_kv8_cache &c, const vkq_kv8_batch &b, int d
     q.rows = dtype == VKQ_F32 || rows <= 8 || steps < dec_ctas(16) * (int64_t)sms ? 8 : 16;
     q.row_tiles = (int)((rows + q.rows - 1) / q.rows);
     q.tiles = b.batch * c.kv_heads * q.row_tiles;
-    // Ranges: one sequence fills the card once (its ranges are alike, and are
-    // joined by one CTA); several, of lengths that the host does not know, get
-    // three times as many, so that the long ones spread.  At least one step a
-    // warp (several sequences: four), and none where the tiles are more than
-    // the workspace's head has counters for.
-    const int64_t slots = dec_ctas(q.rows) * (int64_t)sms, least = kDecWarps * kDecStep * (b.batch > 1 ? 4 : 1);
-    int64_t splits = b.batch > 1 ? (3 * slots + q.tiles - 1) / q.tiles : slots / q.tiles;
-    const int64_t most = (keys + least - 1) / least;
-    if (splits > most) splits = most;
-    if (splits > 128) splits = 128;
-    if (q.tiles > kHeadCounters || splits < 1) splits = 1;
-    int64_t chunk = (keys + splits - 1) / splits;
-    chunk = (chunk + kDecStep - 1) / kDecStep * kDecStep;
+    // Ranges: what is cheapest in units of a CTA's round (a step of each warp),
+    // over the CTAs that the card holds.  A CTA costs its rounds and kStart for
+    // its start and end; each range of a tile kJoin more for the CTA that joins
+    // them.  Several sequences, whose lengths the host does not know, are taken to
+    // be kLong of max_len, and the last CTAs to be alone for kTail of their time.
+    // One range where the tiles are more than the workspace's head has counters
+    // for.  Measured in bfloat16 with 8 KV heads, us in ranges of (most keys a
+    // CTA): 3 contexts of 10,000 to 20,000 tokens 43 (384), 33 (1,024); 2 of 30,000
+    // to 60,000 63 (768), 49 (1,440); 8 of 500 to 3,000 17 (256), 20 (512), 23
+    // (1,024); 32 of 500 to 9,000 85 (4,608), 56 (1,800), 59 (1,500).
+    constexpr double kStart = 3., kJoin = 0.1, kTail = 0.45, kLong = 0.7;
+    const int64_t slots = dec_ctas(q.rows) * (int64_t)sms, steps_all = (keys + kDecStep - 1) / kDecStep;
+    const int64_t most = (steps_all + kDecWarps - 1) / kDecWarps;
+    const double part = b.batch > 1 ? kLong : 1.;
+    int64_t best = 1;
+    double least = 0.;
+    for (int64_t n = 1; n <= 128 && n <= most && (n == 1 || q.tiles <= kHeadCounters); n++) {
+        const double rounds = (double)((steps_all + n - 1) / n) / kDecWarps;
+        const double ctas = (double)q.tiles * (n > 1 ? part * (double)n : 1.);
+        double cost = rounds + kStart;
+        if (b.batch > 1) {
+            const double all = ((double)(q.tiles * most) * part + kStart * ctas) / (double)slots + kTail * rounds;
+            if (all > cost) cost = all;
+        } else {
+            cost *= std::ceil(ctas / (double)slots);
+        }
+        if (n > 1) cost += kJoin * (double)n;
+        if (n == 1 || cost < least) best = n, least = cost;
+    }
+    const int64_t chunk = ((keys + best - 1) / best + kDecStep - 1) / kDecStep * kDecStep;
     q.chunk = (int)chunk;
     q.splits = (int)((keys + chunk - 1) / chunk);
     if (q.splits > 1) {
