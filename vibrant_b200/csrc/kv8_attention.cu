@@ -22,7 +22,7 @@
 // sides of a product, so it drops out.
 //
 // Measured, 40 heads on 8 of D = 128: one context of 200,001 tokens in float32
-// 92 us (4.5 TB/s), 32 of 500 to 9,000 in bfloat16 59 us (3.1 TB/s); one token of
+// 93 us (4.4 TB/s), 32 of 500 to 9,000 in bfloat16 56 us (3.3 TB/s); one token of
 // 1,024 with 16 heads on 2 9 us, a chain of latencies.  The longer ones are bound
 // by the instructions that turn codes into operands, behind them by the loads of
 // two-deep rings: 146 us with two CTAs an SM and 16-row tiles for eight rows.
@@ -36,6 +36,7 @@
 // output's own rounding) and the tile has 16 rows.  Each 16-key product starts from zero and is
 // added to the output in float32 with its vs: the accumulators of the matrix
 // unit round toward zero, which would add up over a long cache.
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 
@@ -522,6 +523,7 @@ static Kv8Plan decode_plan(const vkq_kv8_cache &c, const vkq_kv8_batch &b, int d
     // its start and end; each range of a tile kJoin more for the CTA that joins
     // them.  Several sequences, whose lengths the host does not know, are taken to
     // be kLong of max_len, and the last CTAs to be alone for kTail of their time.
+    // (One sequence's ranges run at once: what is left is rounds / n + kJoin n.)
     // One range where the tiles are more than the workspace's head has counters
     // for.  Measured in bfloat16 with 8 KV heads, us in ranges of (most keys a
     // CTA): 3 contexts of 10,000 to 20,000 tokens 43 (384), 33 (1,024); 2 of 30,000
@@ -530,21 +532,19 @@ static Kv8Plan decode_plan(const vkq_kv8_cache &c, const vkq_kv8_batch &b, int d
     constexpr double kStart = 3., kJoin = 0.1, kTail = 0.45, kLong = 0.7;
     const int64_t slots = dec_ctas(q.rows) * (int64_t)sms, steps_all = (keys + kDecStep - 1) / kDecStep;
     const int64_t most = (steps_all + kDecWarps - 1) / kDecWarps;
-    const double part = b.batch > 1 ? kLong : 1.;
     int64_t best = 1;
-    double least = 0.;
-    for (int64_t n = 1; n <= 128 && n <= most && (n == 1 || q.tiles <= kHeadCounters); n++) {
-        const double rounds = (double)((steps_all + n - 1) / n) / kDecWarps;
-        const double ctas = (double)q.tiles * (n > 1 ? part * (double)n : 1.);
-        double cost = rounds + kStart;
-        if (b.batch > 1) {
-            const double all = ((double)(q.tiles * most) * part + kStart * ctas) / (double)slots + kTail * rounds;
-            if (all > cost) cost = all;
-        } else {
-            cost *= std::ceil(ctas / (double)slots);
+    if (q.tiles <= kHeadCounters && b.batch == 1) {
+        // all at once: least of most / n + kJoin n
+        best = std::min(slots / q.tiles, (int64_t)std::sqrt((double)most / kJoin));
+        best = std::max<int64_t>(1, std::min<int64_t>(best, std::min<int64_t>(most, 128)));
+    } else if (q.tiles <= kHeadCounters) {
+        double least = 0.;
+        for (int64_t n = 1; n <= 128 && n <= most; n += 1 + n / 8) {
+            const double rounds = (double)steps_all / (double)(kDecWarps * n), part = n > 1 ? kLong * (double)n : 1.;
+            const double all = (double)q.tiles * ((double)most * kLong + kStart * part) / (double)slots + kTail * rounds;
+            const double cost = std::max(rounds + kStart, all) + (n > 1 ? kJoin * (double)n : 0.);
+            if (n == 1 || cost < least) best = n, least = cost;
         }
-        if (n > 1) cost += kJoin * (double)n;
-        if (n == 1 || cost < least) best = n, least = cost;
     }
     const int64_t chunk = ((keys + best - 1) / best + kDecStep - 1) / kDecStep * kDecStep;
     q.chunk = (int)chunk;
