@@ -449,7 +449,9 @@ VKQ_API int vkq_rotary(int device, int dtype, const void *x, int64_t x_token_str
  *   VKQ_ROPE_SCALE_NTK:    t_i with the base times factor^(rot_dim / (rot_dim - 2))
  *   VKQ_ROPE_SCALE_YARN:   f_i = t_i / factor * w_i + t_i * (1 - w_i), w_i rising
  *     from 0 to 1 between i = floor(d(beta_fast)) and ceil(d(beta_slow)),
- *     d(b) = rot_dim * ln(orig_len / (2 pi b)) / (2 ln base): pairs that turn
+ *     d(b) = rot_dim * ln(orig_len / (2 pi b)) / (2 ln base), both ends kept
+ *     within 0 .. rot_dim - 1 (the last pair is rot_dim / 2 - 1: with orig_len
+ *     above 2 pi beta_slow base the ramp ends past it): pairs that turn
  *     often within orig_len stay, pairs that do not are interpolated; both
  *     tables are multiplied by attn_factor (0: 0.1 ln(factor) + 1).
  * factor >= 1; orig_len, beta_fast > beta_slow > 0 and attn_factor count for

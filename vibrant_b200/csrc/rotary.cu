@@ -172,7 +172,7 @@ cudaError_t rotary_tables(float *cos_t, float *sin_t, int64_t max_seq, int64_t r
     if (scaling == VKQ_ROPE_SCALE_YARN) {
         const double pi = 3.14159265358979323846;
         auto at = [&](double beta) { return r * std::log((double)orig_len / (2.0 * pi * beta)) / (2.0 * std::log(base)); };
-        const double top = r / 2.0 - 1.0;
+        const double top = r - 1.0;  // the definition's limit: a ramp may end past the last pair, r / 2 - 1
         p.low = std::fmin(std::fmax(std::floor(at(beta_fast)), 0.0), top);
         const double high = std::fmin(std::fmax(std::ceil(at(beta_slow)), 0.0), top);
         p.width = std::fmax(high - p.low, 1e-3);  // equal ends: a step
