@@ -1,0 +1,51 @@
+"""CPU checks of what the 8-bit KV cache's binding keeps and refuses."""
+import contextlib
+import weakref
+
+import pytest
+
+
+@pytest.fixture
+def bare(monkeypatch):
+    """A cache without pool or GPU, whose workspaces are host tensors; capturing[0] says whether a capture runs."""
+    import torch
+    from vibrant_b200 import kv8
+    capturing = [False]
+    monkeypatch.setattr(kv8, "stream_of", lambda device, stream: 7)
+    monkeypatch.setattr(torch.cuda, "stream", lambda stream: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: None)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    c = kv8.Cache.__new__(kv8.Cache)
+    c.device, c._ws, c._captured = torch.device("cpu"), {}, []
+    return c, capturing
+
+
+def test_workspace_of_a_captured_graph_is_kept(bare):
+    """A graph holds the address of the workspace that its capture was given:
+    a later call that needs more must not free it."""
+    c, capturing = bare
+    c._workspace(100, None)
+    capturing[0] = True
+    seen = weakref.ref(c._workspace(100, None))
+    again = c._workspace(200, None)
+    assert again is seen()
+    del again
+    capturing[0] = False
+    more = c._workspace(1 << 22, None)
+    assert more.numel() >= 1 << 22 and int(more.count_nonzero()) == 0
+    assert seen() is not None and seen() is not more
+
+
+def test_workspace_no_capture_has_seen_is_replaced(bare):
+    c, _ = bare
+    seen = weakref.ref(c._workspace(100, None))
+    c._workspace(1 << 22, None)
+    assert seen() is None
+
+
+def test_workspace_does_not_grow_in_a_capture(bare):
+    c, capturing = bare
+    c._workspace(100, None)
+    capturing[0] = True
+    with pytest.raises(RuntimeError):
+        c._workspace(1 << 22, None)

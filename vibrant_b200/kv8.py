@@ -94,6 +94,7 @@ class Cache:
         self.struct = vkq.Kv8CacheStruct(FORMATS[fmt], page_size, kv_heads, head_dim, layers, num_pages,
                                          *(t.data_ptr() for t in buffers))
         self._ws: dict[int, torch.Tensor] = {}
+        self._captured: list[torch.Tensor] = []  # workspaces whose address a graph holds
         self._need: dict[tuple, int] = {}
 
     def _rows(self, t: torch.Tensor, batch: Batch, heads: int | None, name: str) -> tuple[int, int, int]:
@@ -165,24 +166,39 @@ class Cache:
             self._need[key] = need
         return need
 
+    def _capturing(self, stream: torch.cuda.Stream | None) -> bool:
+        if stream is None and torch.cuda.current_device() == self.device.index:
+            return torch.cuda.is_current_stream_capturing()
+        with torch.cuda.stream(torch.cuda.current_stream(self.device) if stream is None else stream):
+            return torch.cuda.is_current_stream_capturing()
+
     def _workspace(self, nbytes: int, stream: torch.cuda.Stream | None) -> torch.Tensor:
-        """A zero-filled workspace of this cache and stream (calls on one stream may share it)."""
+        """A zero-filled workspace of this cache and stream (calls on one stream
+        may share it).  One that a capture has seen lives as long as the cache:
+        its graph keeps the address."""
         key = stream_of(self.device, stream)
         ws = self._ws.get(key)
+        capturing = self._capturing(stream)
         if ws is None or ws.numel() < nbytes:
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("the workspace cannot grow in a stream capture: make the call once before, or "
-                                   "give ws (zero-filled, workspace_bytes(...) long)")
+            if capturing:
+                raise RuntimeError("the workspace cannot grow in a stream capture: make the call once before on the "
+                                   "stream that is captured (torch.cuda.graph(..., stream=s)), or give ws "
+                                   "(zero-filled, workspace_bytes(...) long)")
             with torch.cuda.stream(stream):  # None: the current one
                 ws = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=self.device)
             self._ws[key] = ws
+        if capturing and not any(t is ws for t in self._captured):
+            self._captured.append(ws)
         return ws
 
     def attend(self, layer: int, batch: Batch, q: torch.Tensor, scale: float | None = None, causal: bool = True,
                window: int = 0, out: torch.Tensor | None = None, ws: torch.Tensor | None = None,
                stream: torch.cuda.Stream | None = None) -> torch.Tensor:
         """Attention of the new tokens' q [tokens, heads, head_dim] over the
-        cache (which holds them already); scale defaults to 1 / sqrt(head_dim)."""
+        cache (which holds them already); scale defaults to 1 / sqrt(head_dim).
+        Without ws the cache's own workspace of this stream is used; a graph
+        captured so keeps using it, and must not run at once with another
+        graph of that stream or with calls on it."""
         code = dtype_code(q)
         qp, qs, heads = self._rows(q, batch, None, "q")
         if out is None:
