@@ -54,28 +54,29 @@ struct PagesParams {
 };
 
 // Exclusive sum over the CTA's threads in order; total: over all of them.
-__device__ int block_scan(int v, int &total) {
-    __shared__ int sums[kPlanThreads / 32];
+template <typename T>
+__device__ T block_scan(T v, T &total) {
+    __shared__ T sums[kPlanThreads / 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int x = v;
+    T x = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        const T y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
     }
     if (lane == 31) sums[warp] = x;
     __syncthreads();
     if (warp == 0) {
-        int s = sums[lane];
+        T s = sums[lane];
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, s, o);
+            const T y = __shfl_up_sync(0xffffffffu, s, o);
             if (lane >= o) s += y;
         }
         sums[lane] = s;
     }
     __syncthreads();
-    const int r = x - v + (warp ? sums[warp - 1] : 0);
+    const T r = x - v + (warp ? sums[warp - 1] : 0);
     total = sums[kPlanThreads / 32 - 1];
     __syncthreads();
     return r;
@@ -155,8 +156,8 @@ __global__ void __launch_bounds__(kPlanThreads) extend_kernel(const PagesParams 
         int len = 0, grown = 0;
         bool ok = false;
         const int64_t k = i < p.n ? need(i, len, grown, ok) : 0;
-        int total;
-        const int64_t at = before + block_scan((int)min(k, (int64_t)(1 << 20)), total);
+        int64_t total;  // a row may grow by 2^26 pages, a thousand of them by more than 2^31
+        const int64_t at = before + block_scan(k, total);
         before += total;
         ok = ok && (k == 0 || at + k <= have);
         if (ok) {
