@@ -276,6 +276,17 @@ static int check_attention(const vkq_kv8_cache *cache, int64_t layer, const vkq_
     return VKQ_OK;
 }
 
+// The workspace's size, or an error for bounds whose launch no grid holds.
+static int attention_workspace(const vkq_kv8_cache *cache, const vkq_kv8_batch *batch, int dtype, int64_t heads, int causal,
+                               int64_t window, int device, const char *who, size_t *bytes) {
+    int64_t ctas = 0;
+    *bytes = kv8_attention_workspace(*cache, *batch, dtype, heads, causal, window, device, &ctas);
+    if (ctas <= INT32_MAX) return VKQ_OK;
+    set_error("%s: batch of %lld sequences of up to %lld tokens and %lld heads is too large for one call", who,
+              (long long)batch->batch, (long long)batch->max_tokens, (long long)heads);
+    return VKQ_ERR_UNSUPPORTED;
+}
+
 int vkq_kv8_attention_workspace_bytes(int device, const vkq_kv8_cache *cache, const vkq_kv8_batch *batch, int dtype,
                                       int64_t heads, int causal, int64_t window, size_t *bytes) {
     int st = enter(device);
@@ -286,8 +297,7 @@ int vkq_kv8_attention_workspace_bytes(int device, const vkq_kv8_cache *cache, co
         set_error("%s: null bytes", who);
         return VKQ_ERR_INVALID_ARGUMENT;
     }
-    *bytes = kv8_attention_workspace(*cache, *batch, dtype, heads, causal, window, device);
-    return VKQ_OK;
+    return attention_workspace(cache, batch, dtype, heads, causal, window, device, who, bytes);
 }
 
 int vkq_kv8_attention(int device, const vkq_kv8_cache *cache, int64_t layer, const vkq_kv8_batch *batch, int dtype,
@@ -305,7 +315,8 @@ int vkq_kv8_attention(int device, const vkq_kv8_cache *cache, int64_t layer, con
         return VKQ_ERR_INVALID_ARGUMENT;
     }
     if (batch->tokens == 0) return VKQ_OK;
-    const size_t need = kv8_attention_workspace(*cache, *batch, dtype, heads, causal, window, device);
+    size_t need = 0;
+    if ((st = attention_workspace(cache, batch, dtype, heads, causal, window, device, who, &need))) return st;
     if (!workspace || misaligned(workspace, 16) || workspace_bytes < need) {
         set_error("%s: workspace of %zu bytes, 16-byte aligned, needed (got %zu)", who, need,
                   workspace ? workspace_bytes : (size_t)0);

@@ -577,8 +577,13 @@ static Kv8Plan attention_plan(const vkq_kv8_cache &c, const vkq_kv8_batch &b, in
 }
 
 size_t kv8_attention_workspace(const vkq_kv8_cache &c, const vkq_kv8_batch &b, int dtype, int64_t heads, int causal,
-                               int64_t window, int device) {
+                               int64_t window, int device, int64_t *ctas) {
     const Kv8Plan q = attention_plan(c, b, dtype, heads, causal, window, device);
+    // (few rows: at most 2^16 tiles a sequence and head by many_rows, 128 ranges,
+    // and the grid's other axes are held by the arguments' checks)
+    *ctas = !many_rows(c, b, heads, causal, window) ? (int64_t)q.row_tiles * q.splits
+            : q.splits == 1                         ? q.tiles
+                                                    : q.tiles * std::max(q.splits, q.rows / 32);
     return kWorkspaceCounterHead + (q.part_floats + q.stat_floats) * sizeof(float);
 }
 

@@ -225,8 +225,9 @@ Kv8Plan kv8_prefill_plan(const vkq_kv8_cache &c, const vkq_kv8_batch &b, int dty
 cudaError_t kv8_prefill(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_batch &b, const Kv8AttentionArgs &a,
                         const Kv8Plan &q, cudaStream_t s);
 int kv8_prefill_read_status();
+// Bytes, and in *ctas the largest grid (its x axis) of the call's launches.
 size_t kv8_attention_workspace(const vkq_kv8_cache &c, const vkq_kv8_batch &b, int dtype, int64_t heads, int causal,
-                               int64_t window, int device);
+                               int64_t window, int device, int64_t *ctas);
 cudaError_t kv8_attention(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_batch &b, const Kv8AttentionArgs &a,
                           cudaStream_t s, int device);
 int kv8_attention_read_status();
