@@ -536,10 +536,20 @@ VKQ_API int vkq_kv8_read(int device, const vkq_kv8_cache *cache, int64_t layer, 
  * zeros.  q and out [tokens][heads][head_dim] of dtype, token strides of their
  * own; heads a multiple of kv_heads; scale > 0.  Scores, softmax and sums are
  * float32.  The codes are exact operands of the 16-bit matrix instructions;
- * float32 q and probabilities go through them in two 11-bit parts (error
- * within 1e-5 of sum_j p_j |v_j|, and what float32 scores carry: 2^-20 of
- * scale sum_d |q_d k_jd|), 16-bit ones are rounded once to 11 bits; a p below
- * 2^-39 of its row's largest adds nothing to the sum.  workspace: vkq_kv8_attention_workspace_bytes for these bounds,
+ * float32 q and probabilities go through them in two 11-bit parts, 16-bit
+ * probabilities are rounded once to 11 bits.  With float64's p, the codes c and
+ * scales s of V (v = c s), an output of dimension d is off by at most
+ *   2^-39 F + 1e-5 sum_j p_j |v_jd|  (float32),
+ *   2^-31 F + 2^-10 sum_j p_j |v_jd|  (16-bit), and its own rounding,
+ * and by what float32 scores carry (2^-20 of scale sum_d |q_d k_jd|, of
+ * every p).  F = max_i(p_i s_i) sum_j |c_jd|: in calls of many rows a key
+ * enters the second product as p_j s_j relative to the row's largest, so that
+ * in dimensions where blocks of far larger scales hold zeros, the keys of
+ * small scales lose digits; in calls of few rows F is max_i(p_i) sum_j |v_jd|
+ * and counts 2^-39 for 16-bit too.  Scales s of one row's keys more than
+ * 2^120 apart can cost its softmax the keys of the smaller ones.  workspace:
+ * vkq_kv8_attention_workspace_bytes for these bounds (many rows of long
+ * contexts take some: 4,096 float16 tokens of 200,000 with 40 heads 1.2 GB),
  * 16-byte aligned, zero-filled before its first use; every call leaves it
  * ready for the next one.  Calls that may run at once need separate ones. */
 VKQ_API int vkq_kv8_attention_workspace_bytes(int device, const vkq_kv8_cache *cache, const vkq_kv8_batch *batch,

@@ -17,7 +17,10 @@
 //   O = sum e cv,  l = sum e / vs,  o = O / l:
 // vs goes into the exponent, so that the second product's operand stays
 // within (0, 1], and out of the sum.  Both scales of 16 keys cost a thread two
-// multiplications a tile.
+// multiplications a tile.  The price: e ends, as a float16 operand, at 2^-39 of
+// the row's largest p vs (float32) or 2^-31 (16-bit, whose M may be 2^8 behind),
+// not of its largest p, so a dimension in which blocks of far larger scales
+// hold zeros sees fewer digits of the others.  l comes from the float32 e.
 //
 // 16-bit q: 256 rows in two halves, each with a warpgroup, an issuing warp and
 // two score buffers of 64 keys: the scores of the next 64 keys are computed
