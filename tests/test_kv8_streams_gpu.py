@@ -64,3 +64,69 @@ def test_graphs_captured_with_the_caches_own_workspace():
     for *_, junk in graphs:
         assert all(bool((t == 0x5A).all()) for t in junk)
     assert vkq.device_status(0) == vkq.OK
+
+
+def _calls():
+    """Calls that bring a result [64, 8, 64] of float32 (or several), on a stream that they are given."""
+    import torch
+    from vibrant_b200 import kv8, synth, tensor as vt, vkq
+    rng = np.random.default_rng(22)
+    lens = [90] * 64
+    pool = kh.Pool(64 * 6, 8, 16, 64, "int8", rng)
+    table = kh.table_for(rng, lens, 16, 64 * 6, spare=0)
+    c = _cache(pool)
+    b = kv8.Batch(torch.from_numpy(table).cuda(), _ints(lens))
+    cos, sin = vt.rotary_tables(64, 1e4, 2048)
+    x = torch.randn(64, 8, 64, device="cuda")
+    pos = torch.arange(64, dtype=torch.int32, device="cuda")
+    w = vt.QuantWeight(vkq.Q6_K, 256, 512, synth.weights(vkq.Q6_K, 256, 512, 3))
+    w4 = vt.QuantWeight(vkq.Q4_K, 256, 512, synth.weights(vkq.Q4_K, 256, 512, 4))
+    rows = torch.randn(64, 256, device="cuda")
+    loose = torch.randn(256, 64, device="cuda").t()  # not contiguous
+    return {"rotary": lambda s: (vt.rotary(x, cos, sin, pos, stream=s),),
+            "rotary_tables": lambda s: vt.rotary_tables(32, 1e4, 2048, stream=s),
+            "append": lambda s: (c.append(0, b, x, x, q=x, cos=cos, sin=sin, stream=s),),
+            "read": lambda s: c.read(0, b, pos, pos, stream=s),
+            "attend": lambda s: (c.attend(0, b, x, stream=s),),
+            "matmul": lambda s: (vt.matmul(rows, w, stream=s),),
+            "matmul of a view": lambda s: (vt.matmul(loose, w, stream=s),),
+            "linear_fused": lambda s: tuple(vt.linear_fused(rows[:1].expand(4, 256), [w4], stream=s)),
+            "dequantize": lambda s: (vt.dequantize(w, stream=s),),
+            "dequant_transpose": lambda s: (vt.dequant_transpose(w, stream=s),)}
+
+
+@pytest.mark.parametrize("name", ["rotary", "rotary_tables", "append", "read", "attend", "matmul", "matmul of a view",
+                                  "linear_fused", "dequantize", "dequant_transpose"])
+def test_results_on_another_stream(name):
+    """A result written on `stream` takes no memory that the current stream
+    still reads, and, dropped, is not written again before the current stream
+    has read it."""
+    import torch
+    from vibrant_b200 import vkq
+    call = _calls()[name]
+    want = [t.clone() for t in call(None)]
+    other = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    call(other)  # workspaces and kernels are there
+    torch.cuda.synchronize()
+    held = [torch.full_like(t, 7.0) for t in want]
+    torch.cuda.synchronize()
+    torch.cuda._sleep(100_000_000)  # the current stream is some 50 ms behind
+    seen = [t.clone() for t in held]
+    del held
+    got = call(other)  # runs at once
+    other.synchronize()
+    torch.cuda.synchronize()
+    assert all(bool((t == 7.0).all()) for t in seen)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    # read late on the current stream, dropped, and the same memory asked for on the other one
+    torch.cuda._sleep(100_000_000)
+    late = [t.clone() for t in got]
+    shapes = [(t.shape, t.dtype) for t in got]
+    del got
+    with torch.cuda.stream(other):
+        junk = [torch.full(s, 9.0, dtype=d, device="cuda") for s, d in shapes * 4]
+    other.synchronize()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(late, want)) and len(junk) == 4 * len(want)
+    assert vkq.device_status(0) == vkq.OK

@@ -11,6 +11,8 @@
 
 Every call runs on torch's current stream (or `stream`) and returns without a
 host synchronisation; lengths, page numbers and free pages stay on the device.
+With `stream` the inputs must be ready for it and live until it has used them,
+and a result is ready for another stream once that has waited for this one.
 """
 from __future__ import annotations
 
@@ -19,7 +21,7 @@ import math
 import torch
 
 from . import vkq
-from .tensor import ROPE_LAYOUTS, check_int32, check_tables, dtype_code, stream_of
+from .tensor import ROPE_LAYOUTS, check_int32, check_tables, dtype_code, empty_on, stream_of
 
 FORMATS = {"int8": vkq.KV8_INT8, "e4m3": vkq.KV8_E4M3}
 BLOCK = vkq.KV8_BLOCK
@@ -129,7 +131,7 @@ class Cache:
         if q is not None:
             qp, qs, heads = self._rows(q, batch, None, "q")
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+                q_out = empty_on(q.shape, q.dtype, self.device, stream)
             elif q_out.dtype != q.dtype:
                 raise ValueError("q_out must match q")
             qop, qos, _ = self._rows(q_out, batch, heads, "q_out")
@@ -147,7 +149,7 @@ class Cache:
         check_int32(pos, (seq.shape[0],), "pos", self.device)
         n = seq.shape[0]
         shape = (n, self.kv_heads, self.head_dim)
-        k, v = torch.empty(shape, dtype=dtype, device=self.device), torch.empty(shape, dtype=dtype, device=self.device)
+        k, v = (empty_on(shape, dtype, self.device, stream) for _ in range(2))
         if n:
             vkq.kv8_read(self.struct, layer, batch.bounds(self.page_size), seq.data_ptr(), pos.data_ptr(), n,
                          dtype_code(k), k.data_ptr(), v.data_ptr(), device=self.device.index,
@@ -202,7 +204,7 @@ class Cache:
         code = dtype_code(q)
         qp, qs, heads = self._rows(q, batch, None, "q")
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+            out = empty_on(q.shape, q.dtype, self.device, stream)
         elif out.dtype != q.dtype:
             raise ValueError("out must match q")
         op, os_, _ = self._rows(out, batch, heads, "out")

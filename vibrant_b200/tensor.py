@@ -11,6 +11,26 @@ import torch
 from . import vkq
 
 
+def empty_on(shape, dtype: torch.dtype, device, stream: torch.cuda.Stream | None) -> torch.Tensor:
+    """A result for `stream` to write (None: the current one): its memory comes
+    from that stream, so that nothing queued on the current one still uses it,
+    and once dropped is not reused before what the current one has queued by then."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        out = torch.empty(shape, dtype=dtype, device=device)
+    out.record_stream(torch.cuda.current_stream(out.device))
+    return out
+
+
+def contiguous_on(x: torch.Tensor, stream: torch.cuda.Stream | None) -> torch.Tensor:
+    """x, or its contiguous copy made on `stream` (None: the current one)."""
+    if stream is None or x.is_contiguous():
+        return x.contiguous()
+    with torch.cuda.stream(stream):
+        return x.contiguous()
+
+
 class QuantWeight:
     """A quantized [K, N] weight kept packed in device memory (the raw
     super-block stream, in vibrant's orientation: W[k][n] is value k*N + n)."""
@@ -71,11 +91,11 @@ def linear_fused(x: torch.Tensor, weights: list[QuantWeight], norm_w: torch.Tens
     with x replaced by RMSNorm(x) * norm_w when norm_w is given."""
     if x.dtype != torch.float32 or x.dim() != 2 or any(w.K != x.shape[1] for w in weights):
         raise ValueError(f"x must be float32 [M, K] with K = every weight's K, got {tuple(x.shape)}")
-    x = x.contiguous()
+    x = contiguous_on(x, stream)
     M = x.shape[0]
     n_out = 1 if silu_mul else len(weights)
     if outs is None:
-        outs = [torch.empty((M, weights[i].N), dtype=torch.float32, device=x.device) for i in range(n_out)]
+        outs = [empty_on((M, weights[i].N), torch.float32, x.device, stream) for i in range(n_out)]
     st = stream if stream is not None else torch.cuda.current_stream(x.device)
     vkq.linear_fused(weights[0].qtype, [w.buf.data_ptr() for w in weights], [w.nbytes for w in weights], x.shape[1],
                      [w.N for w in weights], x.data_ptr(), M, [o.data_ptr() for o in outs],
@@ -89,11 +109,11 @@ def matmul(x: torch.Tensor, w: QuantWeight, out: torch.Tensor | None = None, ws:
     """y = x @ W for float32 x [M, K] on the weight's device (vkq_matmul)."""
     if x.dtype != torch.float32 or x.dim() != 2 or x.shape[1] != w.K:
         raise ValueError(f"x must be float32 [M, {w.K}], got {tuple(x.shape)} {x.dtype}")
-    x = x.contiguous()
+    x = contiguous_on(x, stream)
     M = x.shape[0]
     dev = w.device_index
     if out is None:
-        out = torch.empty((M, w.N), dtype=torch.float32, device=x.device)
+        out = empty_on((M, w.N), torch.float32, x.device, stream)
     if ws is None:
         need = workspace_bytes(w.qtype, M, w.K, w.N, dev)
         if path == "gemm":
@@ -111,7 +131,7 @@ def matmul(x: torch.Tensor, w: QuantWeight, out: torch.Tensor | None = None, ws:
 def dequantize(w: QuantWeight, stream=None) -> torch.Tensor:
     """All values of the weight's super-blocks as float32 (vkq_dequantize_f32)."""
     nb = w.nbytes // vkq.BLOCK_BYTES[w.qtype]
-    out = torch.empty(nb * 256, dtype=torch.float32, device=w.buf.device)
+    out = empty_on(nb * 256, torch.float32, w.buf.device, stream)
     st = stream if stream is not None else torch.cuda.current_stream(w.buf.device)
     vkq.dequantize_f32(w.qtype, w.buf.data_ptr(), nb, out.data_ptr(), device=w.device_index, stream=st)
     return out
@@ -119,7 +139,7 @@ def dequantize(w: QuantWeight, stream=None) -> torch.Tensor:
 
 def dequant_transpose(w: QuantWeight, stream=None) -> torch.Tensor:
     """float32 [N, K] transposed copy (vkq_dequant_transpose_f32)."""
-    out = torch.empty((w.N, w.K), dtype=torch.float32, device=w.buf.device)
+    out = empty_on((w.N, w.K), torch.float32, w.buf.device, stream)
     st = stream if stream is not None else torch.cuda.current_stream(w.buf.device)
     vkq.dequant_transpose_f32(w.qtype, w.buf.data_ptr(), w.K, w.N, out.data_ptr(), device=w.device_index,
                               stream=st)
@@ -167,8 +187,7 @@ def rotary_tables(rot_dim: int, base: float, max_seq: int, scaling: str = "none"
                   device="cuda", stream: torch.cuda.Stream | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """cos and sin tables [max_seq, rot_dim / 2] built on the device
     (vkq_rotary_tables_f32); scaling "none", "linear", "ntk" or "yarn"."""
-    cos = torch.empty((max_seq, rot_dim // 2), dtype=torch.float32, device=device)
-    sin = torch.empty_like(cos)
+    cos, sin = (empty_on((max_seq, rot_dim // 2), torch.float32, device, stream) for _ in range(2))
     vkq.rotary_tables_f32(cos.data_ptr(), sin.data_ptr(), max_seq, rot_dim, base, ROPE_SCALINGS[scaling], factor,
                           orig_len, beta_fast, beta_slow, attn_factor, device=cos.device.index, stream=stream_of(cos.device, stream))
     return cos, sin
@@ -189,7 +208,7 @@ def rotary(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: tor
     check_tables(cos, sin, dev)
     check_int32(positions, (T,), "positions", dev)
     if out is None:
-        out = torch.empty((T, H, D), dtype=x.dtype, device=dev)
+        out = empty_on((T, H, D), x.dtype, dev, stream)
         os_ = (H * D, D, 1)
     else:
         os_ = out.stride()
@@ -335,7 +354,7 @@ class PeerGather:
         M = x.shape[0]
         if M > self.m_max:
             raise ValueError(f"M={M} exceeds the group's m_max={self.m_max}")
-        x = x.contiguous()
+        x = contiguous_on(x, stream)
         if ws is None:
             ws = workspace(workspace_bytes(w.qtype, M, w.K, w.width, self.device), self.device)
         st = stream if stream is not None else torch.cuda.current_stream(x.device)
@@ -359,10 +378,10 @@ class PeerGather:
         M = x.shape[0]
         if M > self.m_max or x.dtype != torch.float32:
             raise ValueError("x does not match the group")
-        x = x.contiguous()
+        x = contiguous_on(x, stream)
         local = [] if silu_mul else weights[1:]
         if outs is None:
-            outs = [torch.empty((M, w.N), dtype=torch.float32, device=x.device) for w in local]
+            outs = [empty_on((M, w.N), torch.float32, x.device, stream) for w in local]
         st = stream if stream is not None else torch.cuda.current_stream(x.device)
         vkq.linear_fused_allgather(
             w0.qtype, [w.buf.data_ptr() for w in weights], [w.nbytes for w in weights], w0.K, self.N, w0.lo, w0.hi,
