@@ -49,3 +49,25 @@ def test_workspace_does_not_grow_in_a_capture(bare):
     capturing[0] = True
     with pytest.raises(RuntimeError):
         c._workspace(1 << 22, None)
+
+
+def test_workspace_of_the_products(monkeypatch):
+    """The same for the workspace of the matrix products, which a captured step
+    uses beside the cache's; one made in a capture is the graph's alone."""
+    import torch
+    from vibrant_b200 import tensor as vt
+    capturing, zeros = [False], torch.zeros
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    monkeypatch.setattr(torch, "zeros", lambda n, dtype, device: zeros(n, dtype=dtype))
+    monkeypatch.setattr(vt, "_WS", {})
+    monkeypatch.setattr(vt, "_WS_CAPTURED", [], raising=False)
+    free = weakref.ref(vt.workspace(100, 0))
+    vt.workspace(3 << 20, 0)
+    assert free() is None
+    capturing[0] = True
+    seen = weakref.ref(vt.workspace(100, 0))
+    own = vt.workspace(4 << 20, 0)
+    capturing[0] = False
+    assert vt.workspace(100, 0) is seen() and own is not seen()
+    more = vt.workspace(5 << 20, 0)
+    assert seen() is not None and vt.workspace(4 << 20, 0) is more

@@ -130,3 +130,36 @@ def test_results_on_another_stream(name):
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(late, want)) and len(junk) == 4 * len(want)
     assert vkq.device_status(0) == vkq.OK
+
+
+def test_captured_product_after_its_workspace_grew():
+    """A product split along K, captured with the cached workspace; then one that needs more."""
+    import torch
+    from vibrant_b200 import synth, tensor as vt, vkq
+    w = vt.QuantWeight(vkq.Q6_K, 2048, 512, synth.weights(vkq.Q6_K, 2048, 512, 3))
+    x = torch.randn(2, 2048, device="cuda")
+    side = torch.cuda.Stream()
+    vt._WS.pop((0, 0), None)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = vt.matmul(x, w)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = vt.matmul(x, w)
+    cached = vt._WS.get((0, 0))
+    if cached is not None:
+        size = cached.numel()
+        del cached
+        vt.workspace(4 * size, 0)
+        junk = [torch.full((size,), 0x5A, dtype=torch.uint8, device="cuda") for _ in range(8)]
+        with torch.cuda.stream(side):
+            junk += [torch.full((size,), 0x5A, dtype=torch.uint8, device="cuda") for _ in range(8)]
+        torch.cuda.synchronize()
+    for _ in range(3):
+        out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    if cached_size := vt.workspace_bytes(vkq.Q6_K, 2, 2048, 512, 0):
+        assert cached_size <= size and all(bool((t == 0x5A).all()) for t in junk)

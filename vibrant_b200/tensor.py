@@ -58,6 +58,7 @@ class QuantWeight:
 
 
 _WS: dict[tuple[int, int], torch.Tensor] = {}
+_WS_CAPTURED: list[torch.Tensor] = []
 _WS_NEED: dict[tuple, int] = {}
 
 
@@ -73,14 +74,20 @@ def workspace_bytes(qtype: int, M: int, K: int, N: int, device: int) -> int:
 
 def workspace(nbytes: int, device: int) -> torch.Tensor | None:
     """A zero-filled, cached workspace of at least nbytes on a device (one per
-    device: calls on one stream may share it)."""
+    device: calls on one stream may share it).  One that a stream capture has
+    seen is kept for the graph that holds its address; one that is first needed
+    in a capture belongs to the graph, which fills it again at every replay."""
     if nbytes == 0:
         return None
     key = (device, 0)
     ws = _WS.get(key)
+    capturing = torch.cuda.is_current_stream_capturing()
     if ws is None or ws.numel() < nbytes:
         ws = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=f"cuda:{device}")
-        _WS[key] = ws
+        if not capturing:
+            _WS[key] = ws
+    elif capturing and not any(t is ws for t in _WS_CAPTURED):
+        _WS_CAPTURED.append(ws)
     return ws
 
 
