@@ -51,6 +51,18 @@ def test_workspace_does_not_grow_in_a_capture(bare):
         c._workspace(1 << 22, None)
 
 
+def test_one_batch_with_caches_of_two_page_sizes():
+    """The bound on the lengths is the table's for each cache, not the first one's."""
+    import torch
+    from vibrant_b200 import kv8
+    table, lens = torch.zeros(2, 10, dtype=torch.int32), torch.ones(2, dtype=torch.int32)
+    b = kv8.Batch(table, lens)
+    assert [b.bounds(page).max_len for page in (16, 64, 32)] == [160, 640, 320]
+    b = kv8.Batch(table, lens, max_len=100)
+    assert [b.bounds(page).max_len for page in (16, 64)] == [100, 100]
+    assert kv8.Batch(table, lens, max_len=0).bounds(16).max_len == 0
+
+
 def test_workspace_of_the_products(monkeypatch):
     """The same for the workspace of the matrix products, which a captured step
     uses beside the cache's; one made in a capture is the graph's alone."""

@@ -60,10 +60,9 @@ class Batch:
                                          table.shape[1], n, self.tokens, max_tokens, 0)
 
     def bounds(self, page: int) -> vkq.Kv8BatchStruct:
-        """The struct, its length bound that of the table unless one was given."""
+        """The struct for a cache of this page size: its length bound is that of the table unless one was given."""
         s = self.struct
-        if s.max_len == 0:
-            s.max_len = s.max_pages * page if self.max_len is None else self.max_len
+        s.max_len = s.max_pages * page if self.max_len is None else self.max_len
         return s
 
 
