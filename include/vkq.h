@@ -433,7 +433,8 @@ enum vkq_dtype { VKQ_F32 = 0, VKQ_F16 = 1, VKQ_BF16 = 30 };
  * cos_table and sin_table [max_seq][rot_dim / 2]; in float32, each product and
  * sum rounded on its own, the result rounded once to dtype.  inverse != 0
  * rotates back (s negated; also the gradient of the rotation).  out may be x
- * with the same strides, and may not overlap it in any other way.  A position
+ * with the same strides, and may not overlap it in any other way; its heads
+ * may not overlap one another.  A position
  * outside [0, max_seq) leaves its token unwritten and vkq_device_status then
  * reports VKQ_ERR_INVALID_ARGUMENT.  Element alignment suffices; 16-byte
  * aligned rows and rot_dim a multiple of 16 take the vector path. */

@@ -82,6 +82,20 @@ static int check_heads(const vkq_kv8_cache *c, const vkq_kv8_batch *b, int64_t h
     return VKQ_OK;
 }
 
+// Whether two of the heads at token * a + head * b, of D values each, share
+// values (a, b >= D where there is more than one token or head): only a token
+// more and heads less can meet.
+static bool heads_meet(int64_t tokens, int64_t a, int64_t heads, int64_t b, int64_t D) {
+    if (tokens == 1 || heads == 1 || (a - D) / b >= heads - 1 || (b - D) / a >= tokens - 1) return false;
+    if (tokens > heads) return heads_meet(heads, b, tokens, a, D);
+    for (int64_t d = 1; d < tokens; d++) {  // tokens * heads is bounded: at most 2^20
+        const int64_t k = d * a / b;        // the heads just below and above d tokens on
+        if (k >= 1 && k < heads && d * a - k * b < D) return true;
+        if (k + 1 < heads && (k + 1) * b - d * a < D) return true;
+    }
+    return false;
+}
+
 // Rows of `heads` heads a token: the stride holds them, the elements are aligned.
 static int check_rows(const void *p, int64_t token_stride, int64_t width, int dtype, const char *who, const char *name) {
     if (!p) {
@@ -149,7 +163,8 @@ int vkq_rotary(int device, int dtype, const void *x, int64_t x_token_stride, int
     }
     if (x_token_stride < 0 || x_token_stride > most || x_head_stride < 0 || x_head_stride > most ||
         out_token_stride < 0 || out_token_stride > most || out_head_stride < 0 || out_head_stride > most ||
-        (heads > 1 && out_head_stride < head_dim) || (tokens > 1 && out_token_stride < head_dim)) {
+        (heads > 1 && out_head_stride < head_dim) || (tokens > 1 && out_token_stride < head_dim) ||
+        heads_meet(tokens, out_token_stride, heads, out_head_stride, head_dim)) {
         set_error("vkq_rotary: strides must not be negative, and the output's heads must not overlap");
         return VKQ_ERR_INVALID_ARGUMENT;
     }
