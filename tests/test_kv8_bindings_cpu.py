@@ -51,6 +51,37 @@ def test_workspace_does_not_grow_in_a_capture(bare):
         c._workspace(1 << 22, None)
 
 
+def test_batch_or_workspace_of_another_device(bare, monkeypatch):
+    """Their addresses would mean nothing there: refused before any launch."""
+    import torch
+    from vibrant_b200 import kv8, vkq
+    calls = []
+    for name in ("kv8_append", "kv8_read", "kv8_attention"):
+        monkeypatch.setattr(vkq, name, lambda *a, **k: calls.append(a))
+    monkeypatch.setattr(vkq, "kv8_attention_workspace_bytes", lambda *a, **k: calls.append(a) or 64)
+    c, _ = bare
+    c.page_size, c.kv_heads, c.head_dim, c.struct, c._need = 16, 1, 64, None, {}
+    here, there = (kv8.Batch(torch.zeros(2, 4, dtype=torch.int32, device=d), torch.ones(2, dtype=torch.int32, device=d))
+                   for d in ("cpu", "meta"))
+    x = torch.zeros(2, 1, 64)
+    at = torch.zeros(2, dtype=torch.int32)
+    for call in (lambda b: c.append(0, b, x, x), lambda b: c.read(0, b, at, at), lambda b: c.attend(0, b, x),
+                 lambda b: c.attend(0, b, x, ws=torch.zeros(64)), lambda b: c.workspace_bytes(b, torch.float32, 1)):
+        with pytest.raises(ValueError):
+            call(there)
+        assert not calls
+        call(here)
+        assert calls
+        calls.clear()
+        c._need.clear()
+    for ws in (torch.zeros(64, device="meta"), torch.zeros(64, 2)[:, 0]):
+        with pytest.raises(ValueError):
+            c.attend(0, here, x, ws=ws)
+    assert not calls
+    c.attend(0, here, x, ws=torch.zeros(64))  # float32: 256 bytes
+    assert 256 in calls[0]
+
+
 def test_one_batch_with_caches_of_two_page_sizes():
     """The bound on the lengths is the table's for each cache, not the first one's."""
     import torch

@@ -62,3 +62,16 @@ def test_attention_serves_wide_bounds():
         got = c.attend(0, batch, q.normal_())
         assert bool(((got - v).abs() <= 1e-5 * v.abs()).all())
     assert vkq.device_status(0) == vkq.OK
+
+
+def test_batch_and_workspace_of_the_host_are_refused():
+    import torch
+    from vibrant_b200 import kv8, vkq
+    c, b, q = _small("float32")
+    host = kv8.Batch(b.tensors[0].cpu(), b.tensors[1].cpu())
+    x = q[:, :2].contiguous()
+    for bad in (lambda: c.append(0, host, x, x), lambda: c.attend(0, host, q), lambda: c.read(0, host, *b.tensors[1:2] * 2),
+                lambda: c.attend(0, b, q, ws=torch.zeros(1 << 20, dtype=torch.uint8))):
+        with pytest.raises(ValueError):
+            bad()
+    assert vkq.device_status(0) == vkq.OK

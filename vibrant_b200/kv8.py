@@ -110,6 +110,11 @@ class Cache:
             raise ValueError(f"the heads of a token must be contiguous in {name}")
         return t.data_ptr(), st[0] if s[0] > 1 else s[1] * s[2], s[1]
 
+    def _bounds(self, batch: Batch) -> vkq.Kv8BatchStruct:
+        if batch.device != self.device:
+            raise ValueError(f"the batch is on {batch.device}, the cache on {self.device}")
+        return batch.bounds(self.page_size)
+
     def append(self, layer: int, batch: Batch, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None = None,
                cos: torch.Tensor | None = None, sin: torch.Tensor | None = None, layout: str = "interleaved",
                q_out: torch.Tensor | None = None, stream: torch.cuda.Stream | None = None) -> torch.Tensor | None:
@@ -136,7 +141,7 @@ class Cache:
             qop, qos, _ = self._rows(q_out, batch, heads, "q_out")
         if batch.tokens == 0:
             return q_out
-        vkq.kv8_append(self.struct, layer, batch.bounds(self.page_size), code, kp, ks, vp, vs, qp or None, qs,
+        vkq.kv8_append(self.struct, layer, self._bounds(batch), code, kp, ks, vp, vs, qp or None, qs,
                        qop or None, qos, heads, _ptr(cos), _ptr(sin), seq, rot, ROPE_LAYOUTS[layout],
                        device=self.device.index, stream=stream_of(self.device, stream))
         return q_out
@@ -150,14 +155,14 @@ class Cache:
         shape = (n, self.kv_heads, self.head_dim)
         k, v = (empty_on(shape, dtype, self.device, stream) for _ in range(2))
         if n:
-            vkq.kv8_read(self.struct, layer, batch.bounds(self.page_size), seq.data_ptr(), pos.data_ptr(), n,
+            vkq.kv8_read(self.struct, layer, self._bounds(batch), seq.data_ptr(), pos.data_ptr(), n,
                          dtype_code(k), k.data_ptr(), v.data_ptr(), device=self.device.index,
                          stream=stream_of(self.device, stream))
         return k, v
 
     def workspace_bytes(self, batch: Batch, dtype: torch.dtype, heads: int, causal: bool = True, window: int = 0) -> int:
         """vkq_kv8_attention_workspace_bytes, memoised."""
-        s = batch.bounds(self.page_size)
+        s = self._bounds(batch)
         key = (dtype, heads, causal, window, s.batch, s.max_tokens, s.max_len)
         need = self._need.get(key)
         if need is None:
@@ -211,8 +216,11 @@ class Cache:
             return out
         if ws is None:
             ws = self._workspace(self.workspace_bytes(batch, q.dtype, heads, causal, window), stream)
-        vkq.kv8_attention(self.struct, layer, batch.bounds(self.page_size), code, qp, qs, op, os_, heads,
-                          1.0 / math.sqrt(self.head_dim) if scale is None else scale, ws.data_ptr(), ws.numel(),
+        elif ws.device != self.device or not ws.is_contiguous():
+            raise ValueError(f"ws must be contiguous on {self.device}")
+        vkq.kv8_attention(self.struct, layer, self._bounds(batch), code, qp, qs, op, os_, heads,
+                          1.0 / math.sqrt(self.head_dim) if scale is None else scale, ws.data_ptr(),
+                          ws.numel() * ws.element_size(),
                           causal, window, device=self.device.index, stream=stream_of(self.device, stream))
         return out
 
