@@ -379,11 +379,6 @@ cudaError_t attention_decode_rope(const float *q, const float *k_new, const floa
     return attention_launch(p, batch, head_dim, true, s);
 }
 
-int attention_read_status() {
-    int v = 0, zero = 0;
-    if (cudaMemcpyFromSymbol(&v, g_attn_status, sizeof(int)) != cudaSuccess) return -1;
-    cudaMemcpyToSymbol(g_attn_status, &zero, sizeof(int));
-    return v;
-}
+int *attention_status_word() { return status_word(g_attn_status); }
 
 }  // namespace vkq

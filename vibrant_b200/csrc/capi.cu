@@ -723,27 +723,28 @@ int vkq_device_status(int device, int *code) {
     }
     cudaError_t e = cudaDeviceSynchronize();
     if (e != cudaSuccess) return check_launch(e, "cudaDeviceSynchronize");
-    int g = gemv_read_status();
-    const int g2 = gemm_read_status();
-    const int g3 = gemv_tc_read_status();
-    const int g4 = gemv_strip_read_status();
-    const int g5 = elem_read_status();
-    const int g6 = attention_read_status();
-    const int g7 = rotary_read_status();
-    const int g8 = kv8_read_status();
-    const int g9 = kv8_attention_read_status();
-    const int g10 = kv8_pages_read_status();
-    if (g == 0) g = g2;
-    if (g == 0) g = g3;
-    if (g == 0) g = g4;
-    if (g == 0) g = g5;
-    if (g == 0) g = g6;
-    if (g == 0) g = g7;
-    if (g == 0) g = g8;
-    if (g == 0) g = g9;
-    if (g == 0) g = g10;
-    if (g < 0 || g2 < 0 || g3 < 0 || g4 < 0 || g5 < 0 || g6 < 0 || g7 < 0 || g8 < 0 || g9 < 0 ||
-        g10 < 0) {
+    // the words come back together: a synchronous copy each would be 12 us of host time
+    int *const words[] = {gemv_status_word(), gemm_status_word(),   gemv_tc_status_word(), gemv_strip_status_word(),
+                          elem_status_word(), attention_status_word(), rotary_status_word(),  kv8_status_word(),
+                          kv8_attention_status_word(), kv8_prefill_status_word(), kv8_pages_status_word()};
+    constexpr int n = sizeof(words) / sizeof(words[0]);
+    static std::mutex mu;
+    static int *host = nullptr;  // pinned
+    std::lock_guard<std::mutex> lock(mu);
+    if (!host) e = cudaHostAlloc(reinterpret_cast<void **>(&host), n * sizeof(int), cudaHostAllocPortable);
+    for (int i = 0; i < n && e == cudaSuccess; i++)
+        e = words[i] ? cudaMemcpyAsync(host + i, words[i], sizeof(int), cudaMemcpyDeviceToHost, cudaStreamLegacy)
+                     : cudaErrorInvalidSymbol;
+    const cudaError_t done = cudaStreamSynchronize(cudaStreamLegacy);
+    if (e == cudaSuccess) e = done;
+    int g = 0;
+    for (int i = 0; i < n && e == cudaSuccess; i++) {
+        if (host[i] == 0) continue;
+        if (g == 0) g = host[i];
+        e = cudaMemset(words[i], 0, sizeof(int));
+    }
+    if (g != 0 && e == cudaSuccess) e = cudaStreamSynchronize(cudaStreamLegacy);
+    if (e != cudaSuccess) {
         set_error("cannot read the device status word");
         return VKQ_ERR_CUDA;
     }

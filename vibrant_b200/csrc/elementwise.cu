@@ -97,12 +97,7 @@ __global__ void __launch_bounds__(256) rope_kernel(const float2 *x, float2 *out,
     }
 }
 
-int elem_read_status() {
-    int v = 0, zero = 0;
-    if (cudaMemcpyFromSymbol(&v, g_elem_status, sizeof(int)) != cudaSuccess) return -1;
-    cudaMemcpyToSymbol(g_elem_status, &zero, sizeof(int));
-    return v;
-}
+int *elem_status_word() { return status_word(g_elem_status); }
 
 // dst[0..n) = src[0..n), src being pinned host memory that the device reads
 // through its mapping.  The loads do not depend on the preceding kernel and

@@ -901,11 +901,6 @@ int gemm_launch(const GemvShape &s, const void *w, int64_t w_bytes, const float 
     return 0;
 }
 
-int gemm_read_status() {
-    int v = 0, zero = 0;
-    if (cudaMemcpyFromSymbol(&v, g_gemm_status, sizeof(int)) != cudaSuccess) return -1;
-    cudaMemcpyToSymbol(g_gemm_status, &zero, sizeof(int));
-    return v;
-}
+int *gemm_status_word() { return status_word(g_gemm_status); }
 
 }  // namespace vkq

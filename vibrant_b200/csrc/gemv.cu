@@ -1157,11 +1157,6 @@ int gemv_launch_noalloc(const GemvShape &s, const void *w, int64_t w_bytes, cons
     return gemv_launch(s, w, w_bytes, x, y, base, kNoAllocScratchBytes, stream, device);
 }
 
-int gemv_read_status() {
-    int v = 0, zero = 0;
-    if (cudaMemcpyFromSymbol(&v, g_gemv_status, sizeof(int)) != cudaSuccess) return -1;
-    cudaMemcpyToSymbol(g_gemv_status, &zero, sizeof(int));
-    return v;
-}
+int *gemv_status_word() { return status_word(g_gemv_status); }
 
 }  // namespace vkq

@@ -719,11 +719,6 @@ int gemv_strip_gather(const GemvShape &s, const void *w, int64_t w_bytes, const 
     return gemv_strip_multi((int)s.M, s.K, &seg, 1, false, x, nullptr, 0.f, stream, device, &g);
 }
 
-int gemv_strip_read_status() {
-    int v = 0, zero = 0;
-    if (cudaMemcpyFromSymbol(&v, g_strip_status, sizeof(int)) != cudaSuccess) return -1;
-    cudaMemcpyToSymbol(g_strip_status, &zero, sizeof(int));
-    return v;
-}
+int *gemv_strip_status_word() { return status_word(g_strip_status); }
 
 }  // namespace vkq

@@ -823,11 +823,6 @@ int gemv_tc_launch(const GemvShape &s, const TcLayout &L, const void *w, int64_t
     return 0;
 }
 
-int gemv_tc_read_status() {
-    int v = 0, zero = 0;
-    if (cudaMemcpyFromSymbol(&v, g_tc_status, sizeof(int)) != cudaSuccess) return -1;
-    cudaMemcpyToSymbol(g_tc_status, &zero, sizeof(int));
-    return v;
-}
+int *gemv_tc_status_word() { return status_word(g_tc_status); }
 
 }  // namespace vkq

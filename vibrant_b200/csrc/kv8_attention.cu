@@ -627,12 +627,6 @@ cudaError_t kv8_attention(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_b
     return cudaLaunchKernelExC(&cfg, fn, args);
 }
 
-int kv8_attention_read_status() {
-    int v = 0, zero = 0;
-    if (cudaMemcpyFromSymbol(&v, g_kv8_attn_status, sizeof(int)) != cudaSuccess) return -1;
-    cudaMemcpyToSymbol(g_kv8_attn_status, &zero, sizeof(int));
-    const int w = kv8_prefill_read_status();
-    return w < 0 || v == 0 ? w : v;
-}
+int *kv8_attention_status_word() { return status_word(g_kv8_attn_status); }
 
 }  // namespace vkq

@@ -512,11 +512,6 @@ cudaError_t kv8_read(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_batch 
     return launch(fn, (n + p.rows - 1) / p.rows, kReadThreads, &p, s);
 }
 
-int kv8_read_status() {
-    int v = 0, zero = 0;
-    if (cudaMemcpyFromSymbol(&v, g_kv8_status, sizeof(int)) != cudaSuccess) return -1;
-    cudaMemcpyToSymbol(g_kv8_status, &zero, sizeof(int));
-    return v;
-}
+int *kv8_status_word() { return status_word(g_kv8_status); }
 
 }  // namespace vkq

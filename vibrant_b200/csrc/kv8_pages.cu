@@ -459,11 +459,6 @@ cudaError_t kv8_copy_pages(const vkq_kv8_cache &c, const int *src, const int *ds
     return launch_move(c, src, dst, nullptr, n, false, s, device);
 }
 
-int kv8_pages_read_status() {
-    int v = 0, zero = 0;
-    if (cudaMemcpyFromSymbol(&v, g_kv8_pages_status, sizeof(int)) != cudaSuccess) return -1;
-    cudaMemcpyToSymbol(g_kv8_pages_status, &zero, sizeof(int));
-    return v;
-}
+int *kv8_pages_status_word() { return status_word(g_kv8_pages_status); }
 
 }  // namespace vkq

@@ -1031,11 +1031,6 @@ cudaError_t kv8_prefill(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_bat
     return cudaLaunchKernelExC(&cfg, join, args);
 }
 
-int kv8_prefill_read_status() {
-    int v = 0, zero = 0;
-    if (cudaMemcpyFromSymbol(&v, g_kv8_prefill_status, sizeof(int)) != cudaSuccess) return -1;
-    cudaMemcpyToSymbol(g_kv8_prefill_status, &zero, sizeof(int));
-    return v;
-}
+int *kv8_prefill_status_word() { return status_word(g_kv8_prefill_status); }
 
 }  // namespace vkq

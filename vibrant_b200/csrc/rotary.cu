@@ -184,11 +184,6 @@ cudaError_t rotary_tables(float *cos_t, float *sin_t, int64_t max_seq, int64_t r
     return launch((const void *)rotary_tables_kernel, blocks, 256, &p, s);
 }
 
-int rotary_read_status() {
-    int v = 0, zero = 0;
-    if (cudaMemcpyFromSymbol(&v, g_rotary_status, sizeof(int)) != cudaSuccess) return -1;
-    cudaMemcpyToSymbol(g_rotary_status, &zero, sizeof(int));
-    return v;
-}
+int *rotary_status_word() { return status_word(g_rotary_status); }
 
 }  // namespace vkq

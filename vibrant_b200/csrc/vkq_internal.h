@@ -10,6 +10,14 @@
 
 namespace vkq {
 
+// The device address of a source file's status word (NULL: it cannot be had).
+// vkq_device_status reads all of them and clears those that are set.
+template <typename Word>
+inline int *status_word(Word &word) {
+    void *p = nullptr;
+    return cudaGetSymbolAddress(&p, word) == cudaSuccess ? static_cast<int *>(p) : nullptr;
+}
+
 int device_sm_count(int device);
 // Raises a kernel's dynamic shared-memory limit on the current device to at
 // least `smem` bytes (with `carveout`, also its preferred carveout to the
@@ -66,7 +74,7 @@ int gemv_launch(const GemvShape &s, const void *w, int64_t w_bytes, const float 
 // workspace argument, nothing allocated); see vkq_gemv_noalloc.
 int gemv_launch_noalloc(const GemvShape &s, const void *w, int64_t w_bytes, const float *x, float *y,
                         cudaStream_t stream, int device);
-int gemv_read_status();
+int *gemv_status_word();
 // Selects the kernel of plain GEMVs: 0 automatic, 1 CUDA cores (gemv.cu), 2
 // tensor cores (gemv_tc.cu), 3 column strips (gemv_strip.cu); returns the
 // previous choice.
@@ -85,7 +93,7 @@ bool gemv_tc_fits(const GemvShape &s, const TcLayout &L, int device);
 size_t gemv_tc_workspace_bytes(const GemvShape &s, const TcLayout &L, int device);
 int gemv_tc_launch(const GemvShape &s, const TcLayout &L, const void *w, int64_t w_bytes, const float *x, float *y,
                    int64_t y_ld, void *ws, size_t ws_bytes, cudaStream_t stream, int device);
-int gemv_tc_read_status();
+int *gemv_tc_status_word();
 
 // Q4_K column-strip GEMV (gemv_strip.cu), 1 <= M <= 4, for stored rows that
 // start on a super-block boundary: row k of the weight is rs / 256 blocks,
@@ -118,7 +126,7 @@ int gemv_strip_multi(int M, int64_t K, const StripSeg *segs, int nseg, bool silu
 bool gemv_strip_gather_fits(const GemvShape &s, const GatherArgs &g, int device);
 int gemv_strip_gather(const GemvShape &s, const void *w, int64_t w_bytes, const float *x, const GatherArgs &g,
                       cudaStream_t stream, int device);
-int gemv_strip_read_status();  // reads and clears the column-strip kernel's device status word
+int *gemv_strip_status_word();  // of the column-strip kernel
 
 // fp32 GEMV for weights in the upstream GGUF orientation (gemv_rows.cu):
 // y[m][n] = sum_k x[m][k] * W[n][k], W[n][k] = value n*K + k; K % 256 == 0,
@@ -130,7 +138,7 @@ cudaError_t gemv_rows_launch(int qtype, const void *w, int64_t K, int64_t N, con
 size_t gemm_workspace_bytes(const GemvShape &s, int device);
 int gemm_launch(const GemvShape &s, const void *w, int64_t w_bytes, const float *x, float *y, void *ws,
                 size_t ws_bytes, cudaStream_t stream, int device);
-int gemm_read_status();  // reads and clears this TU's device status word (synchronous)
+int *gemm_status_word();
 
 // SiLU(gate) * up and row-wise RMSNorm (elementwise.cu); 16-byte aligned buffers.
 cudaError_t silu_mul(const float *gate, const float *up, float *out, int64_t n, cudaStream_t s, int device);
@@ -146,18 +154,18 @@ cudaError_t attention_decode(const float *q, const float *kc, const float *vc, f
 // [batch][kv_heads][D] before RoPE; rotates q and k_new at positions[b],
 // stores the rotated k_new and v_new at row len - 1 of the caches and
 // attends over rows 0 .. len-1.  A position outside [0, max_seq) skips its
-// sequence and sets the status word attention_read_status() returns.
+// sequence and sets the status word vkq_device_status returns.
 cudaError_t attention_decode_rope(const float *q, const float *k_new, const float *v_new, const float *cos_t,
                                   const float *sin_t, const int *positions, float *kc, float *vc, float *o,
                                   int64_t batch, int64_t heads, int64_t kv_heads, int64_t len, int64_t cache_len,
                                   int64_t head_dim, int64_t max_seq, cudaStream_t s);
-int attention_read_status();  // reads and clears the attention kernels' status word
+int *attention_status_word();
 // Rotary position embedding over interleaved pairs (elementwise.cu): x and
 // out [rows][head_dim] with rows = batch * heads * seq, seq the fastest;
 // tables [max_seq][head_dim / 2]; 8-byte aligned x, out.
 cudaError_t rope(const float *x, float *out, const float *cos_t, const float *sin_t, const int *positions,
                  int64_t rows, int64_t seq, int64_t head_dim, int64_t max_seq, cudaStream_t s, int device);
-int elem_read_status();  // reads and clears the elementwise kernels' status word
+int *elem_status_word();
 // dst[0..n) = src[0..n) from pinned host memory through its device mapping
 // (elementwise.cu), as a kernel that takes part in programmatic dependent launch.
 cudaError_t stage_in(const float *src_mapped, float *dst, int64_t n, cudaStream_t s);
@@ -178,7 +186,7 @@ cudaError_t rotary(const RotaryArgs &a, cudaStream_t s, int device);
 cudaError_t rotary_tables(float *cos_t, float *sin_t, int64_t max_seq, int64_t rot_dim, double base, int scaling,
                           double factor, int64_t orig_len, double beta_fast, double beta_slow, double attn_factor,
                           cudaStream_t s, int device);
-int rotary_read_status();
+int *rotary_status_word();
 
 // The 8-bit paged KV cache: append and read-back (kv8_cache.cu), attention
 // (kv8_attention.cu), page operations (kv8_pages.cu).  Arguments are checked
@@ -199,7 +207,7 @@ cudaError_t kv8_append(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_batc
                        cudaStream_t s, int device);
 cudaError_t kv8_read(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_batch &b, const int *seq, const int *pos,
                      int64_t n, int dtype, void *k_out, void *v_out, cudaStream_t s);
-int kv8_read_status();
+int *kv8_status_word();
 struct Kv8AttentionArgs {
     int dtype;
     const void *q;
@@ -224,13 +232,13 @@ Kv8Plan kv8_prefill_plan(const vkq_kv8_cache &c, const vkq_kv8_batch &b, int dty
                          int64_t window, int sms);
 cudaError_t kv8_prefill(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_batch &b, const Kv8AttentionArgs &a,
                         const Kv8Plan &q, cudaStream_t s);
-int kv8_prefill_read_status();
+int *kv8_prefill_status_word();
 // Bytes, and in *ctas the largest grid (its x axis) of the call's launches.
 size_t kv8_attention_workspace(const vkq_kv8_cache &c, const vkq_kv8_batch &b, int dtype, int64_t heads, int causal,
                                int64_t window, int device, int64_t *ctas);
 cudaError_t kv8_attention(const vkq_kv8_cache &c, int64_t layer, const vkq_kv8_batch &b, const Kv8AttentionArgs &a,
                           cudaStream_t s, int device);
-int kv8_attention_read_status();
+int *kv8_attention_status_word();
 size_t kv8_pages_workspace(const vkq_kv8_cache &c, const vkq_kv8_seqs &q);
 cudaError_t kv8_extend(const vkq_kv8_cache &c, const vkq_kv8_seqs &q, const int *slots, const int *add, int64_t n,
                        int *done, void *ws, cudaStream_t s);
@@ -240,7 +248,7 @@ cudaError_t kv8_free(const vkq_kv8_cache &c, const vkq_kv8_seqs &q, const int *s
                      cudaStream_t s);
 cudaError_t kv8_compact(const vkq_kv8_cache &c, const vkq_kv8_seqs &q, int *used, void *ws, cudaStream_t s, int device);
 cudaError_t kv8_copy_pages(const vkq_kv8_cache &c, const int *src, const int *dst, int64_t n, cudaStream_t s, int device);
-int kv8_pages_read_status();
+int *kv8_pages_status_word();
 
 // Makes `device` current and checks that the kernels can run on it; returns a
 // vkq_status code (capi.cu).  check_launch turns a CUDA error into one.
