@@ -13,8 +13,8 @@ def bare(monkeypatch):
     capturing = [False]
     monkeypatch.setattr(kv8, "stream_of", lambda device, stream: 7)
     monkeypatch.setattr(torch.cuda, "stream", lambda stream: contextlib.nullcontext())
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: None)
-    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: None)
+    monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: capturing[0])
     c = kv8.Cache.__new__(kv8.Cache)
     c.device, c._ws, c._captured = torch.device("cpu"), {}, []
     return c, capturing

@@ -56,13 +56,16 @@ class Batch:
         self.device = dev
         self.tokens = n if tokens is None else tokens
         self.max_len = max_len
+        self._page = 0  # the page size that struct.max_len is for
         self.struct = vkq.Kv8BatchStruct(_ptr(table), _ptr(lens), _ptr(slots), _ptr(cu_tokens), table.shape[0],
                                          table.shape[1], n, self.tokens, max_tokens, 0)
 
     def bounds(self, page: int) -> vkq.Kv8BatchStruct:
         """The struct for a cache of this page size: its length bound is that of the table unless one was given."""
         s = self.struct
-        s.max_len = s.max_pages * page if self.max_len is None else self.max_len
+        if page != self._page:
+            s.max_len = s.max_pages * page if self.max_len is None else self.max_len
+            self._page = page
         return s
 
 
@@ -162,7 +165,9 @@ class Cache:
 
     def workspace_bytes(self, batch: Batch, dtype: torch.dtype, heads: int, causal: bool = True, window: int = 0) -> int:
         """vkq_kv8_attention_workspace_bytes, memoised."""
-        s = self._bounds(batch)
+        return self._needed(self._bounds(batch), dtype, heads, causal, window)
+
+    def _needed(self, s: vkq.Kv8BatchStruct, dtype: torch.dtype, heads: int, causal: bool, window: int) -> int:
         key = (dtype, heads, causal, window, s.batch, s.max_tokens, s.max_len)
         need = self._need.get(key)
         if need is None:
@@ -173,8 +178,8 @@ class Cache:
         return need
 
     def _capturing(self, stream: torch.cuda.Stream | None) -> bool:
-        if stream is None and torch.cuda.current_device() == self.device.index:
-            return torch.cuda.is_current_stream_capturing()
+        if stream is None and torch._C._cuda_getDevice() == self.device.index:  # asked for on every call: 0.4 us
+            return torch._C._cuda_isCurrentStreamCapturing()
         with torch.cuda.stream(torch.cuda.current_stream(self.device) if stream is None else stream):
             return torch.cuda.is_current_stream_capturing()
 
@@ -214,14 +219,17 @@ class Cache:
         op, os_, _ = self._rows(out, batch, heads, "out")
         if batch.tokens == 0:
             return out
+        s = self._bounds(batch)
         if ws is None:
-            ws = self._workspace(self.workspace_bytes(batch, q.dtype, heads, causal, window), stream)
-        elif ws.device != self.device or not ws.is_contiguous():
-            raise ValueError(f"ws must be contiguous on {self.device}")
-        vkq.kv8_attention(self.struct, layer, self._bounds(batch), code, qp, qs, op, os_, heads,
-                          1.0 / math.sqrt(self.head_dim) if scale is None else scale, ws.data_ptr(),
-                          ws.numel() * ws.element_size(),
-                          causal, window, device=self.device.index, stream=stream_of(self.device, stream))
+            ws = self._workspace(self._needed(s, q.dtype, heads, causal, window), stream)
+            size = ws.numel()
+        else:
+            if ws.device != self.device or not ws.is_contiguous():
+                raise ValueError(f"ws must be contiguous on {self.device}")
+            size = ws.numel() * ws.element_size()
+        vkq.kv8_attention(self.struct, layer, s, code, qp, qs, op, os_, heads,
+                          1.0 / math.sqrt(self.head_dim) if scale is None else scale, ws.data_ptr(), size, causal, window,
+                          device=self.device.index, stream=stream_of(self.device, stream))
         return out
 
     def copy_pages(self, src: torch.Tensor, dst: torch.Tensor, stream: torch.cuda.Stream | None = None) -> None:
