@@ -492,7 +492,9 @@ typedef struct vkq_kv8_cache {
  * out (cu_tokens NULL: row b alone) and stand at positions lens - n .. lens - 1.
  * max_tokens bounds the new tokens of one sequence, max_len the lengths (the
  * host's plan goes by them; the lengths themselves stay on the device, so a
- * captured graph can be replayed while they grow).  A row, a length, a token
+ * captured graph can be replayed while they grow; bounds far above what is
+ * there cost time, because the work is cut by them).  The rows of a call are
+ * distinct where it writes (vkq_kv8_append).  A row, a length, a token
  * range or a page outside its bounds makes no access: vkq_kv8_append leaves
  * the sequence (or the block) out, vkq_kv8_attention gives NaN for the rows
  * that it concerns, and vkq_device_status reports VKQ_ERR_INVALID_ARGUMENT. */
@@ -514,8 +516,9 @@ typedef struct vkq_kv8_batch {
  * a <= m * s_new (kept within [2^-64, 2^63]); a block that holds older tokens
  * keeps its scale if that is larger, else its older codes are rounded again to
  * s_new.  Codes are round-to-nearest-even of x / s, saturating; a NaN is
- * stored as 0.  Blocks of no new token are not touched.  Element alignment
- * suffices. */
+ * stored as 0.  Blocks of no new token are not touched.  With tables, a
+ * sequence longer than max_seq is left out and reported, and its rows of q_out
+ * stay unwritten.  Element alignment suffices. */
 VKQ_API int vkq_kv8_append(int device, const vkq_kv8_cache *cache, int64_t layer, const vkq_kv8_batch *batch, int dtype,
                            const void *k, int64_t k_token_stride, const void *v, int64_t v_token_stride,
                            const void *q, int64_t q_token_stride, void *q_out, int64_t q_out_token_stride,
@@ -543,7 +546,7 @@ VKQ_API int vkq_kv8_read(int device, const vkq_kv8_cache *cache, int64_t layer, 
  *   2^-39 F + 1e-5 sum_j p_j |v_jd|  (float32),
  *   2^-31 F + 2^-10 sum_j p_j |v_jd|  (16-bit), and its own rounding,
  * and by what float32 scores carry (2^-20 of scale sum_d |q_d k_jd|, of
- * every p).  F = max_i(p_i s_i) sum_j |c_jd|: in calls of many rows a key
+ * every p; a |q_d| below 2^-17 of its row's largest counts as that much).  F = max_i(p_i s_i) sum_j |c_jd|: in calls of many rows a key
  * enters the second product as p_j s_j relative to the row's largest, so that
  * in dimensions where blocks of far larger scales hold zeros, the keys of
  * small scales lose digits; in calls of few rows F is max_i(p_i) sum_j |v_jd|
@@ -568,8 +571,11 @@ VKQ_API int vkq_kv8_attention(int device, const vkq_kv8_cache *cache, int64_t la
  * vkq_device_status reports VKQ_ERR_INVALID_ARGUMENT) and run on the device
  * without a host read.  done (NULL: not wanted) receives 1 for a listed row
  * that was served and 0 for one that was left as it was, because it is invalid
- * or too few pages are free.  workspace: vkq_kv8_pages_workspace_bytes,
- * 16-byte aligned, zero-filled before its first use, left ready by every call. */
+ * or too few pages are free.  lens belongs to these calls: a length made
+ * shorter by hand leaves the pages past it held for good.  workspace:
+ * vkq_kv8_pages_workspace_bytes, 16-byte aligned, zero-filled before its first
+ * use, left ready by every call for the next one on a pool and bookkeeping of
+ * the same sizes. */
 typedef struct vkq_kv8_seqs {
     int32_t *table, *lens, *refs;
     int64_t rows, max_pages;
@@ -602,9 +608,10 @@ VKQ_API int vkq_kv8_copy_pages(int device, const vkq_kv8_cache *cache, const int
                                int64_t n, void *stream);
 
 /* Reads and clears the device-side status word of this library on a device
- * (set when a bounded wait inside a kernel gave up, or a peer was out of
- * step).  Synchronizes with the device.  *code receives VKQ_OK,
- * VKQ_ERR_DEVICE_TIMEOUT or VKQ_ERR_PEER. */
+ * (set when a bounded wait inside a kernel gave up, a peer was out of step, or
+ * an index on the device was out of bounds).  Synchronizes with the device.
+ * *code receives VKQ_OK, VKQ_ERR_DEVICE_TIMEOUT, VKQ_ERR_PEER or
+ * VKQ_ERR_INVALID_ARGUMENT. */
 VKQ_API int vkq_device_status(int device, int *code);
 
 #ifdef __cplusplus

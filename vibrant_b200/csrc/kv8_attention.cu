@@ -14,8 +14,10 @@
 // order, so results do not depend on timing.
 //
 // The products run on m16n8k16 with float16 operands: codes are exact in
-// float16 (kv8_widen), and a decode step has some 16 rows, which would leave a
-// 128-row tcgen05 tile nearly empty (many_rows has both sides measured).  Each
+// float16 (kv8_widen), and a decode step has some 16 rows, which leave a
+// 128-row tcgen05 tile with q's rows in it nearly empty (many_rows has both
+// sides measured; the operands exchanged, keys in the 128 rows and q's rows as
+// columns, would fill it and have not been built).  Each
 // lane's operand columns are chosen so that its 16-byte loads from shared memory
 // hold whole fragments: column k of a K step is dimension 16 (c + 4 h) + 4 w +
 // ..., column n of a V tile t is dimension (D / 8) n + t; the same order on both
@@ -522,7 +524,8 @@ static Kv8Plan decode_plan(const vkq_kv8_cache &c, const vkq_kv8_batch &b, int d
     // over the CTAs that the card holds.  A CTA costs its rounds and kStart for
     // its start and end; each range of a tile kJoin more for the CTA that joins
     // them.  Several sequences, whose lengths the host does not know, are taken to
-    // be kLong of max_len, and the last CTAs to be alone for kTail of their time.
+    // be kLong of max_len, and the last CTAs to be alone for kTail of their time
+    // (31 of 500 to 9,000 with max_len 4 and 16 times the longest: 81, 85, 132 us).
     // (One sequence's ranges run at once: what is left is rounds / n + kJoin n.)
     // One range where the tiles are more than the workspace's head has counters
     // for.  Measured in bfloat16 with 8 KV heads, us in ranges of (most keys a
@@ -563,6 +566,9 @@ static Kv8Plan decode_plan(const vkq_kv8_cache &c, const vkq_kv8_batch &b, int d
 // 32,768, 20 rows 48 / 59 (50 / 77), 40 rows 63 / 58 (73 / 74), 80 rows 92 / 56
 // (139 / 73); one of 2,048 and 2 KV heads, 64 rows 13 / 18 (14 / 18), 192 rows
 // (786,432 pairs of a row and a key) 22 / 21 (16 / 18), 512 rows 25 / 21 (26 / 20).
+// One rule for a call: single tokens beside a chunk take the chunk's tiles, and
+// two calls are faster then.  One chunk of 512 and 31 tokens of 500 to 9,000, 40
+// heads on 8: 256 (363) together, 54 + 81 (87 + 82) apart.
 static bool many_rows(const vkq_kv8_cache &c, const vkq_kv8_batch &b, int64_t heads, int causal, int64_t window) {
     const int64_t g = heads / c.kv_heads, rows = b.max_tokens * g;
     const double pairs = (double)(rows * c.kv_heads * b.batch) * (double)seen_keys(b, rows, g, causal, window);

@@ -399,8 +399,8 @@ static PagesParams pages_params(const vkq_kv8_cache &c, const vkq_kv8_seqs &q, c
     return p;
 }
 
-// The mover's grid: `moves` at most, two CTAs of 256 threads an SM to hide a
-// page's latency behind another's.
+// The mover's grid: a CTA a piece of `moves` at most, and no more than the eight
+// of 256 threads that an SM holds, to hide a page's latency behind another's.
 static cudaError_t launch_move(const vkq_kv8_cache &c, const int *from, const int *to, const int *count, int64_t moves,
                                bool holes, cudaStream_t s, int device) {
     MoveParams p{};

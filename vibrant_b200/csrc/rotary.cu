@@ -10,8 +10,9 @@
 // kRotHeads heads of the token, because reading them again for every head
 // would be as many bytes from L1 as the heads themselves.  8,191 tokens of 40
 // heads of 128, whole rows: 26 us in bfloat16 interleaved (6.3 TB/s), 33 halved,
-// 52 in float32 (6.5 TB/s); value by value, for other alignments, 119.  One
-// token 2 us either way.
+// 52 in float32 (6.5 TB/s).  Rows or rot_dim that are no whole pieces go value by
+// value, a pair a thread with entries of its own: 119 us, left so as the rarer
+// case.  One token 2 us either way.
 #include <cmath>
 #include <cstdint>
 
