@@ -552,8 +552,8 @@ VKQ_API int vkq_kv8_read(int device, const vkq_kv8_cache *cache, int64_t layer, 
  * small scales lose digits; in calls of few rows F is max_i(p_i) sum_j |v_jd|
  * and counts 2^-39 for 16-bit too.  Scales s of one row's keys more than
  * 2^120 apart can cost its softmax the keys of the smaller ones.  workspace:
- * vkq_kv8_attention_workspace_bytes for these bounds (many rows of long
- * contexts take some: 4,096 float16 tokens of 200,000 with 40 heads 1.2 GB),
+ * vkq_kv8_attention_workspace_bytes for these bounds (chunks of long contexts
+ * take some: 4,096 tokens of 200,000 with 40 heads 256 MB),
  * 16-byte aligned, zero-filled before its first use; every call leaves it
  * ready for the next one.  Calls that may run at once need separate ones. */
 VKQ_API int vkq_kv8_attention_workspace_bytes(int device, const vkq_kv8_cache *cache, const vkq_kv8_batch *batch,

@@ -38,3 +38,48 @@ def test_sums_of_one_sign_over_long_contexts(dtype, tokens, n):
                         "float32": (2.0 ** -18, 0.0, 1e-5)}[dtype]
     assert abs(float(rel.mean())) <= bias, float(rel.mean())
     assert float(rel.abs().max()) <= half + rest
+
+
+@pytest.mark.parametrize("dtype,tokens,n,window", [
+    ("float16", 900, 40000, 0), ("float16", 70, 40000, 0), ("float16", 900, 50000, 33000), ("float16", 4096, 120000, 0),
+    ("bfloat16", 900, 150000, 0), ("float32", 300, 40000, 0)])
+def test_rising_and_falling_scores_over_long_contexts(dtype, tokens, n, window):
+    """Scores that rise (even heads) or fall (odd ones) by 60 over the context, V
+    of both signs: the running maximum moves all the way, or not at all.  Some
+    rows against float64 and the bound that the header states."""
+    import torch
+    from vibrant_b200 import kv8, vkq
+    H, D, page = 40, 128, 64
+    pages = -(-n // page)
+    g = torch.Generator(device="cuda").manual_seed(n + tokens)
+    c = kv8.Cache(1, pages, page, 1, D)
+    c.v.random_(0, 256, generator=g)
+    c.v[c.v == 128] = 1  # -128 is no code
+    codes = torch.randint(-40, 41, (pages * page, D), generator=g, device="cuda")
+    codes[:, 0] = torch.arange(pages * page, device="cuda") * 120 // (pages * page)
+    order = torch.randperm(pages, generator=g, device="cuda")
+    c.k[0, order, 0] = codes.to(torch.int8).view(torch.uint8).view(pages, page, D)
+    ints = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    b = kv8.Batch(order.int().view(1, -1), ints([n]), cu_tokens=ints([0, tokens]), tokens=tokens, max_tokens=tokens, max_len=n)
+    q = torch.randn(tokens, H, D, generator=g, device="cuda")
+    q[:, 0::2, 0], q[:, 1::2, 0] = 500.0, -500.0
+    q = q.to(getattr(torch, dtype))
+    scale = 1e-3
+    got = c.attend(0, b, q, scale=scale, window=window)
+    assert torch.equal(got, c.attend(0, b, q, scale=scale, window=window)) and vkq.device_status(0) == vkq.OK
+    k, v = codes[:n].double(), c.v[0, order, 0].view(torch.int8).flatten(0, 1)[:n].double()
+    scale = float(torch.tensor(scale, dtype=torch.float32))
+    for row in (0, tokens // 2, tokens - 1):
+        at = n - tokens + row
+        lo = max(at - window + 1, 0) if window else 0
+        kk, vv, qq = k[lo:at + 1], v[lo:at + 1], q[row].double()
+        p = torch.softmax(qq @ kk.T * scale, dim=1)
+        out, mass = p @ vv, p @ vv.abs()
+        size = (qq.abs() @ kk.abs().T * scale).amax(dim=1, keepdim=True)
+        floor = p.amax(dim=1, keepdim=True) * vv.abs().sum(dim=0)
+        tol = (1e-5 + 2.0 ** -20 * size) * mass
+        if dtype == "float32":
+            tol += 2.0 ** -39 * floor
+        else:
+            tol += 2.0 ** -31 * floor + 2.0 ** -10 * mass + (2.0 ** -8 if dtype == "bfloat16" else 2.0 ** -11) * 1.001 * out.abs()
+        assert bool(((got[row].double() - out).abs() <= tol).all())

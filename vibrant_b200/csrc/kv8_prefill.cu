@@ -25,9 +25,9 @@
 // 16-bit q: 256 rows in two halves, each with a warpgroup, an issuing warp and
 // two score buffers of 64 keys: the scores of the next 64 keys are computed
 // while a warpgroup works on the ones before, and a K or V tile is converted
-// once for 256 rows.  e is rounded to 11 bits; the output stays in TMEM over a
-// range of keys, and M is raised (and the output rescaled) only when the
-// maximum grew by more than 2^8, which the operand's range allows.
+// once for 256 rows.  e is rounded to 11 bits; the output stays in TMEM, and M
+// is raised (and the output rescaled) only when the maximum grew by more than
+// 2^8, which the operand's range allows.
 // float32 q: 128 rows; q and e are split into two 11-bit parts, so a tile
 // takes the same four products, every key tile's output starts from zero, and
 // warpgroup 1 adds it to float32 registers while warpgroup 0 works on the next
@@ -35,8 +35,8 @@
 //
 // The matrix unit's accumulators round toward zero, and that adds up: values of
 // one sign lose 6.2e-9 of their sum a key (measured: 4.1e-4 over 66,700 keys).
-// That is why float32 adds tile by tile, and a range of 16-bit q holds at
-// most kRangeF16 or kRangeBf16 keys, whose parts the join adds in float32.
+// That is why float32 adds tile by tile, and 16-bit q moves its output to
+// float32 sums in the workspace every kMoveF16 or kMoveBf16 keys.
 //
 // Row tiles go from each sequence's last (which sees most keys) to its first, so
 // that the longest start first.  Few tiles are split along the keys, and their parts
@@ -76,12 +76,15 @@ constexpr int kPreSub = 64;                       // keys whose scores a thread 
 constexpr int kPreRing = 3;  // float16 tiles
 constexpr int kPreRaw = 3;   // tiles of codes
 constexpr uint32_t kPrePolls = 1u << 27;
-// Keys of a range of 16-bit q: 1.0e-4 and 4.1e-4 lost at most, a fifth and a
-// tenth of the rounding of a float16 or bfloat16 output (half a unit, 2^-11 and
-// 2^-8).  Measured, 4,096 tokens of 200,000, 40 heads on 8 of D = 128: float16
-// loses 7.5e-5 in 13 ranges, 24.8 ms, and lost 4.1e-4 in the 3 that the cost
-// alone would choose, 20.7 ms; bfloat16 22.4 ms in 4.
-constexpr int64_t kRangeF16 = 16384, kRangeBf16 = 65536;
+// Keys after which 16-bit q moves its output out of TMEM: 1.0e-4 and 4.1e-4 lost
+// at most, a fifth and a tenth of the rounding of a float16 or bfloat16 output
+// (half a unit, 2^-11 and 2^-8).  Measured, 4,096 float16 tokens of 200,000, 40
+// heads on 8 of D = 128: 9.2e-5 lost and 20.8 ms, 4.1e-4 and 20.7 ms without;
+// ranges of so many keys instead took 24.8 ms and five times the workspace.
+constexpr int kMoveF16 = 16384, kMoveBf16 = 65536;
+// and the score warps' passes that they are
+template <typename T> constexpr int kMovePasses = kMoveF16 / kPreSub;
+template <> constexpr int kMovePasses<__nv_bfloat16> = kMoveBf16 / kPreSub;
 // registers a thread of warpgroups 0 and 1, of 2, of 3: at most 4 x 128 in all
 // (float32: warpgroup 1 holds a row's output)
 template <bool SPLIT> struct PreRegs {
@@ -357,6 +360,14 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
     int row_token = 0;
     bool there = false;
     float m = -INFINITY, l = 0.f;
+    float moved_m = -INFINITY;  // the M of what the row's output has moved to the workspace
+    // the row's sums there, four dimensions at ROWS float4 a step (16-bit q, and the parts of ranges)
+    auto moved = [&]() { return reinterpret_cast<float4 *>(p.part + (tile * p.splits + split) * ROWS * D) + row; };
+    auto add_moved = [&](float (&x)[8], const float4 *d, float k) {
+        const float4 a = d[0], b = d[ROWS];
+        x[0] = fmaf(a.x, k, x[0]), x[1] = fmaf(a.y, k, x[1]), x[2] = fmaf(a.z, k, x[2]), x[3] = fmaf(a.w, k, x[3]);
+        x[4] = fmaf(b.x, k, x[4]), x[5] = fmaf(b.y, k, x[5]), x[6] = fmaf(b.z, k, x[6]), x[7] = fmaf(b.w, k, x[7]);
+    };
     if (wg < 2) {
         there = r0 + row < rows_all;
         row_token = there ? (r0 + row) / p.g : 0;
@@ -721,7 +732,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
                 } else {
                     // raised only when e would pass 2^8: the output stays as it is otherwise
                     const bool raise = mx > m + 8.f;
-                    if (__any_sync(0xffffffffu, raise)) {
+                    const bool move = i > 0 && i % kMovePasses<T> == 0;
+                    if (move || __any_sync(0xffffffffu, raise)) {
                         if (raise) {
                             al = ex2p(m - mx);
                             m = mx;
@@ -730,14 +742,33 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
                             ok = wait_warp(bar(TE + hf), (i - 1) & 1);  // the output of the keys before
                             if (!ok) break;
                             fence_after();
+                            const uint32_t o0 = my + kO + 128u * hf;
+                            if (!move) {
 #pragma unroll 1
-                            for (int c = 0; c < D / 8; c++) {
-                                uint32_t o[8];
-                                tmem_ld8(o, my + kO + 128u * hf + 8u * c);
-                                tmem_wait_ld(o);
+                                for (int c = 0; c < D / 8; c++) {
+                                    uint32_t o[8];
+                                    tmem_ld8(o, o0 + 8u * c);
+                                    tmem_wait_ld(o);
 #pragma unroll
-                                for (int u = 0; u < 8; u++) o[u] = __float_as_uint(__uint_as_float(o[u]) * al);
-                                tmem_st8(my + kO + 128u * hf + 8u * c, o);
+                                    for (int u = 0; u < 8; u++) o[u] = __float_as_uint(__uint_as_float(o[u]) * al);
+                                    tmem_st8(o0 + 8u * c, o);
+                                }
+                            } else {
+                                const float old = moved_m == m ? 1.f : ex2p(moved_m - m);
+                                moved_m = m;
+                                float4 *d = moved();
+#pragma unroll 1
+                                for (int c = 0; c < D / 8; c++, d += 2 * ROWS) {
+                                    uint32_t o[8];
+                                    tmem_ld8(o, o0 + 8u * c);
+                                    tmem_wait_ld(o);
+                                    float x[8];
+#pragma unroll
+                                    for (int u = 0; u < 8; u++) x[u] = __uint_as_float(o[u]) * al, o[u] = 0u;
+                                    if (i > kMovePasses<T>) add_moved(x, d, old);
+                                    d[0] = make_float4(x[0], x[1], x[2], x[3]), d[ROWS] = make_float4(x[4], x[5], x[6], x[7]);
+                                    tmem_st8(o0 + 8u * c, o);
+                                }
                             }
                         }
                     }
@@ -833,6 +864,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
             if (bad_flag || abort_flag) l = nan;
             put_stat(m, l);
             const float inv = l == 0.f ? 0.f : 1.f / l;
+            const bool add = 2 * n > kMovePasses<T>;
+            const float old = moved_m == m ? 1.f : ex2p(moved_m - m);
 #pragma unroll 1
             for (int i = 0; i < D / 32; i++) {
                 uint32_t o[32];
@@ -848,6 +881,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv8_prefill_kernel(const Prefi
                     float v[8];
 #pragma unroll
                     for (int u = 0; u < 8; u++) v[u] = __uint_as_float(o[c + u]);
+                    if (add) add_moved(v, moved() + (32 * i + c) / 4 * ROWS, old);
                     put(32 * i + c, v, inv);
                 }
             }
@@ -960,21 +994,17 @@ Kv8Plan kv8_prefill_plan(const vkq_kv8_cache &c, const vkq_kv8_batch &b, int dty
     if (causal && window > 0) seen = (double)keys;
     int64_t best = most;  // a range's key tiles
     double least = 0.;
-    // at least as many ranges as the accumulators' rounding asks for
-    const int64_t longest = dtype == VKQ_F32 ? most : (dtype == VKQ_F16 ? kRangeF16 : kRangeBf16) / kPreKeys;
-    const int64_t fewest = (most + longest - 1) / longest;
-    for (int64_t n = fewest; (n <= 64 || n == fewest) && n <= most; n++) {
+    for (int64_t n = 1; n <= 64 && n <= most; n++) {
         const int64_t tiles = (most + n - 1) / n, ranges = (most + tiles - 1) / tiles, ctas = q.tiles * ranges;
         double cost = (double)((ctas + sms - 1) / sms) * ((double)tiles * seen / (double)keys + kStart);
         if (ranges > 1) cost += kJoin + (double)(ctas * q.rows * c.head_dim) * kPart;
-        if (n == fewest || cost < least) best = tiles, least = cost;
+        if (n == 1 || cost < least) best = tiles, least = cost;
     }
     q.chunk = (int)(best * kPreKeys);
     q.splits = (int)((most + best - 1) / best);
-    if (q.splits > 1) {
-        q.part_floats = (size_t)(q.tiles * q.splits * q.rows * c.head_dim);
-        q.stat_floats = (size_t)(q.tiles * q.splits * q.rows * 2);
-    }
+    const bool moves = dtype != VKQ_F32 && q.chunk > (dtype == VKQ_F16 ? kMoveF16 : kMoveBf16);
+    if (q.splits > 1 || moves) q.part_floats = (size_t)(q.tiles * q.splits * q.rows * c.head_dim);
+    if (q.splits > 1) q.stat_floats = (size_t)(q.tiles * q.splits * q.rows * 2);
     return q;
 }
 
